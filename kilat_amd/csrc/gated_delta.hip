@@ -1,0 +1,1108 @@
+// gated_delta.hip — the gated delta rule (include/kdelta.h).
+//
+// Per head, S_t = a_t (S_{t-1} - b_t k_t (k_t' S_{t-1})) + b_t k_t v_t', o_t = scale S_t' q_t.
+// What token t writes is k_t u_t' with u_t = b_t (v_t - a_t S_{t-1}' k_t), so over a chunk
+// of 64 tokens that starts from S, with G_i = g_1 + .. + g_i inside the chunk,
+//
+//     (I + A) U = R,   R_i = b_i (v_i - e^{G_i} S' k_i),   A_ij = b_i e^{G_i - G_j} k_i.k_j  (j < i)
+//     o_i = scale e^{G_i} S' q_i + sum_{j <= i} P_ij u_j,  P_ij = scale e^{G_i - G_j} q_i.k_j
+//     S  <- e^{G_64} S + sum_j e^{G_64 - G_j} k_j u_j'
+//
+// T = (I + A)^-1 and P do not depend on S: prep() computes them for every chunk
+// at once.  chain() then goes through a sequence's chunks; a wavefront keeps
+// 16 columns of S in registers and needs no other wavefront: every product
+// above leaves those columns where they are.
+#include "matrix.h"
+
+#include "kdelta.h"
+
+namespace kd {
+namespace delta {
+
+constexpr int C = 64;       // tokens of a chunk
+constexpr int NX = 3;       // terms of a 32-bit value that reaches the state or a gradient
+constexpr int kFrag = 512;  // bfloat16 values of one operand tile (64 lanes of 8)
+// An operand with zeros above its diagonal of 16-row tiles: tiles of rows 0, 1 need
+// the first 32 inner indices only (transposed: rows 2, 3 the last 32 only).
+constexpr int kTri = 6;
+__host__ __device__ constexpr int tri_lower(int mt, int kb) { return mt < 2 ? mt : 2 * (mt - 1) + kb; }
+__host__ __device__ constexpr int tri_upper(int mt, int kb) { return mt < 2 ? 2 * mt + kb : mt + 2; }
+
+// Terms of P, and products kept, in what reaches o only.
+template <typename T>
+constexpr int kOutTerms = sizeof(T) == 4 ? 3 : 2;
+template <typename T>
+constexpr int kOutOrder = sizeof(T) == 4 ? 2 : 1;
+
+// Per token of a chunk, floats.
+enum Vec { V_BG, V_BETA, V_SINCE, V_LEFT, V_G, V_GLOW, V_COUNT };
+
+struct Args {
+  const void *q, *k, *v;
+  const float *g, *beta;
+  const int32_t* cu;
+  const float* init;
+  int64_t qb, qh, qn, kb, kh, kn, vb, vh, vn, gb, gh, gn, bb, bh, bn;
+  int64_t N, sequences, tiles;
+  int Hk, H, Dk, Dv, group;
+  float scale;
+  bool vec_k, vec_q, vec_v;  // rows start on four elements
+  // scratch, by tile and head
+  __bf16* keys;    // [tiles][Hk][3][4 KB][NI][kFrag]: K, its transpose, Q (backward: its transpose)
+  __bf16* tris;    // [tiles][H][kTri * (NX + kOutTerms)][kFrag]: T and P (backward: transposed)
+  float* vecs;     // [tiles][H][V_COUNT][C]
+  float* states;   // saved: [tiles][H][Dk][Dv], S at the chunk's start
+  float* us;       // saved: [tiles][H][C][Dv]
+  void* o;
+  int64_t ob, oh, on;
+  bool vec_o;
+  float* final;
+  // backward
+  const void* d_o;
+  int64_t dob, doh, don;
+  bool vec_do;
+  const float* d_final;
+  float* d_init;
+  float* dstates;  // [tiles][H][Dk][Dv], the gradient of the state at the chunk's end
+  float* drs;      // [tiles][H][C][Dv], the gradient of R
+  void *dq, *dk, *dv;
+  int64_t dqb, dqh, dqn, dkb, dkh, dkn, dvb, dvh, dvn;
+  bool vec_dq, vec_dk;
+  float *dg, *dbeta;
+};
+
+// Where a tile's operands are.
+template <int KB, int NI>
+__device__ __forceinline__ __bf16* key_tiles(const Args& a, int64_t tile, int hk) {
+  return a.keys + ((tile * a.Hk + hk) * 3) * (int64_t)(4 * KB * NI * kFrag);
+}
+template <typename T>
+__device__ __forceinline__ __bf16* tri_tiles(const Args& a, int64_t tile, int h) {
+  return a.tris + (tile * a.H + h) * (int64_t)(kTri * (NX + kOutTerms<T>)*kFrag);
+}
+__device__ __forceinline__ float* vec_of(const Args& a, int64_t tile, int h) {
+  return a.vecs + (tile * a.H + h) * (int64_t)(V_COUNT * C);
+}
+
+template <int N>
+__device__ __forceinline__ Terms<N> load_terms(const __bf16* p, int lane) {
+  Terms<N> r;
+#pragma unroll
+  for (int n = 0; n < N; ++n) r.t[n] = *reinterpret_cast<const bf16x8*>(p + n * kFrag + lane * 8);
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void store_terms(__bf16* p, int lane, const Terms<N>& x) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) *reinterpret_cast<bf16x8*>(p + n * kFrag + lane * 8) = x.t[n];
+}
+
+// e^x for a difference of sums of log decays (positive for a growing state only).
+__device__ __forceinline__ float fade(double x) {
+  const float hi = (float)x, e = expf(hi);
+  return fmaf(e, (float)(x - (double)hi), e);
+}
+
+// --------------------------------------------------------------------------
+// prep: T, P and the operand tiles of one chunk and value head
+// --------------------------------------------------------------------------
+// Grid (tiles, H), four wavefronts; wavefront w has tokens 16w..16w+15 of the chunk.
+// BWD: T, P and Q transposed, as the backward reads them.
+//
+// log decays are added up in 64 bits: the sums over a chunk can be far larger than
+// the differences that count.  One below -128 is taken as -128: e^-128 is 0 in 32 bits,
+// and no difference becomes inf - inf.
+template <typename T, int KB, bool BWD>
+__global__ __launch_bounds__(256) void prep(Args a) {
+  constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>;
+  constexpr int LD = C + 4;
+  __shared__ __bf16 kq[2][4 * KB * NI * kFrag];  // K and Q
+  __shared__ float As[C * LD], Ts[C * LD];
+  __shared__ double Gs[C];
+  __shared__ float bs[C];
+  const int64_t tile = blockIdx.x;
+  const int h = blockIdx.y, hk = h / a.group;
+  const int w = threadIdx.x / 64, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  if (!BWD)
+    zero_outside<C>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, threadIdx.x, 256);
+  else
+    zero_outside<C>(a.cu, a.sequences, tile, a.N, (T*)a.dv + h * a.dvh, a.dvn, a.Dv, threadIdx.x, 256);
+  const TileOf at = tile_of<C>(a.cu, a.sequences, tile, a.N);
+  const int64_t left_rows = at.rows.n - at.index * C;
+  if (left_rows <= 0) return;
+  const int n = left_rows < C ? (int)left_rows : C;
+  const int64_t row0 = at.rows.first + at.index * C;
+  if (w == 0) {
+    const bool in = lane < n;
+    double G = 0.;
+    float b = 0.f;
+    if (in) {
+      const float x = a.g[at.rows.batch * a.gb + h * a.gh + (row0 + lane) * a.gn];
+      G = x < -128.f ? -128. : (double)x;
+      b = a.beta[at.rows.batch * a.bb + h * a.bh + (row0 + lane) * a.bn];
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const double y = __shfl_up(G, d);
+      if (lane >= d) G += y;
+    }
+    Gs[lane] = G;
+    bs[lane] = b;
+    const double all = __shfl(G, 63);
+    float* vec = vec_of(a, tile, h);
+    const float since = fade(G);
+    vec[V_BG * C + lane] = b * since;
+    vec[V_BETA * C + lane] = b;
+    vec[V_SINCE * C + lane] = since;
+    vec[V_LEFT * C + lane] = fade(all - G);
+    vec[V_G * C + lane] = (float)G;
+    vec[V_GLOW * C + lane] = (float)(G - (double)(float)G);
+  }
+  // Operand tiles of K and Q: lane (m, g) has token 16w + m.
+  const int t = 16 * w + m;
+  const T* krow = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + (row0 + t) * a.kn;
+  const T* qrow = (const T*)a.q + at.rows.batch * a.qb + hk * a.qh + (row0 + t) * a.qn;
+  Terms<NI> kt[KB], qt[KB];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    float x[8];
+    load8(krow, 32 * kb, g, t < n ? a.Dk : 0, a.vec_k, x);
+    kt[kb] = split<NI>(x);
+    load8(qrow, 32 * kb, g, t < n ? a.Dk : 0, a.vec_q, x);
+    qt[kb] = split<NI>(x);
+    store_terms<NI>(kq[0] + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
+    store_terms<NI>(kq[1] + (w * KB + kb) * NI * kFrag, lane, qt[kb]);
+  }
+  __syncthreads();
+  if (h % a.group == 0) {
+    __bf16* out = key_tiles<KB, NI>(a, tile, hk);
+    constexpr int kAll = 4 * KB * NI * kFrag;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      store_terms<NI>(out + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
+      if (!BWD) store_terms<NI>(out + 2 * kAll + (w * KB + kb) * NI * kFrag, lane, qt[kb]);
+    }
+    // Transposed: rows are channels, inner indices tokens.
+    for (int f = w; f < 4 * KB; f += 4) {
+      const int d = 16 * (f / 2) + m, tb = 32 * (f & 1);
+      const int src = (d / 32) * NI * kFrag + (d & 3) + ((d >> 4) & 1) * 4;
+      const int sl = 16 * ((d >> 2) & 3);
+#pragma unroll
+      for (int x = 0; x < (BWD ? 2 : 1); ++x) {
+        Terms<NI> r;
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int tok = tb + 4 * g + (i & 3) + 16 * (i >> 2);
+            r.t[j][i] = kq[x][(tok >> 4) * KB * NI * kFrag + src + j * kFrag + (sl + (tok & 15)) * 8];
+          }
+        store_terms<NI>(out + (1 + x) * kAll + f * NI * kFrag, lane, r);
+      }
+    }
+  }
+  // A for tokens i of this wavefront, lane m = column j (read by rows below).
+  __bf16* tri = tri_tiles<T>(a, tile, h);
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (jt <= w) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) acc = product<2>(kt[kb], load_terms<NI>(kq[0] + (jt * KB + kb) * NI * kFrag, lane), acc);
+    }
+    const int j = 16 * jt + m;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = 16 * w + 4 * g + x;
+      As[i * LD + j] = j < i ? bs[i] * fade(Gs[i] - Gs[j]) * acc[x] : 0.f;
+    }
+  }
+  // P: rows i of this wavefront (BWD: transposed, rows j of this wavefront).
+#pragma unroll
+  for (int kb2 = 0; kb2 < 2; ++kb2) {
+    if (BWD ? kb2 < w / 2 : kb2 > w / 2) continue;
+    f32x4 p[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int ot = 2 * kb2 + x;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const Terms<NI> y = load_terms<NI>(kq[BWD ? 1 : 0] + (ot * KB + kb) * NI * kFrag, lane);
+        acc = product<2>(y, BWD ? kt[kb] : qt[kb], acc);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int mine = 16 * w + m, other = 16 * ot + 4 * g + r;
+        const int i = BWD ? other : mine, j = BWD ? mine : other;
+        p[x][r] = j <= i ? a.scale * fade(Gs[i] - Gs[j]) * acc[r] : 0.f;
+      }
+    }
+    const int f = BWD ? tri_upper(w, kb2) : tri_lower(w, kb2);
+    store_terms<NO>(tri + (kTri * NX + f * NO) * kFrag, lane, split<NO>(p[0], p[1]));
+  }
+  __syncthreads();
+  // T = (I + A)^-1.  The 16 x 16 diagonal blocks by forward substitution, a column per
+  // lane; below them T_ij = -T_ii sum_k A_ik T_kj, in 32-bit products.
+  {
+    float x[16];
+    const float* A = As + (16 * w) * LD + 16 * w;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == m ? 1.f : 0.f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) s = fmaf(-A[i * LD + j], x[j], s);
+      x[i] = s;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i / 4 == g) Ts[(16 * w + i) * LD + 16 * w + m] = x[i];
+    for (int jt = w + 1; jt < 4; ++jt)  // zeros above
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Ts[(16 * w + 4 * g + i) * LD + 16 * jt + m] = 0.f;
+  }
+  __syncthreads();
+  {
+    f32x4 col[4];  // T's tiles of columns 16w.., rows w..3
+#pragma unroll
+    for (int x = 0; x < 4; ++x) col[0][x] = Ts[(16 * w + 4 * g + x) * LD + 16 * w + m];
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+      const int it = w + d;
+      if (it < 4) {
+        f32x4 y = {0.f, 0.f, 0.f, 0.f}, z = y;
+#pragma unroll
+        for (int e = 0; e < d; ++e) {
+          const float* r = As + (16 * it + m) * LD + 16 * (w + e) + 4 * g;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) y = __builtin_amdgcn_mfma_f32_16x16x4f32(r[x], col[e][x], y, 0, 0, 0);
+        }
+        const float* r = Ts + (16 * it + m) * LD + 16 * it + 4 * g;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) z = __builtin_amdgcn_mfma_f32_16x16x4f32(r[x], -y[x], z, 0, 0, 0);
+        col[d] = z;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) Ts[(16 * it + 4 * g + x) * LD + 16 * w + m] = z[x];
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int kb2 = 0; kb2 < 2; ++kb2) {
+    if (BWD ? kb2 < w / 2 : kb2 > w / 2) continue;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int o = 32 * kb2 + 4 * g + (i & 3) + 16 * (i >> 2);
+      x[i] = BWD ? Ts[o * LD + t] : Ts[t * LD + o];
+    }
+    const int f = BWD ? tri_upper(w, kb2) : tri_lower(w, kb2);
+    store_terms<NX>(tri + f * NX * kFrag, lane, split<NX>(x));
+  }
+}
+
+// --------------------------------------------------------------------------
+// chain: the chunks of one sequence and head, 16 columns of the state per wavefront
+// --------------------------------------------------------------------------
+// A chunk token by token, for the chunks that hold a value that is not finite: a
+// product with the zeros of T and P would carry it to earlier tokens.
+template <typename T, int KB, bool SAVE>
+__device__ __noinline__ void chunk_by_token(const Args& a, const Rows& rows, int64_t row0, int n, int h, int col,
+                                            int64_t tile, f32x4 (&S)[2 * KB]) {
+  const int hk = h / a.group, lane = threadIdx.x & 63, g = lane >> 4;
+  for (int t = 0; t < n; ++t) {
+    const T* krow = (const T*)a.k + rows.batch * a.kb + hk * a.kh + (row0 + t) * a.kn;
+    const T* qrow = (const T*)a.q + rows.batch * a.qb + hk * a.qh + (row0 + t) * a.qn;
+    const float dec = expf(a.g[rows.batch * a.gb + h * a.gh + (row0 + t) * a.gn]);
+    const float b = a.beta[rows.batch * a.bb + h * a.bh + (row0 + t) * a.bn];
+    float x = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      const f32x4 k = load4(krow + 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g, a.vec_k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (16 * dt + 4 * g + i < a.Dk) {
+          S[dt][i] *= dec;
+          x = fmaf(k[i], S[dt][i], x);
+        }
+      }
+    }
+    x = group_sum(x);
+    const float v = col < a.Dv ? (float)((const T*)a.v)[rows.batch * a.vb + h * a.vh + (row0 + t) * a.vn + col] : 0.f;
+    const float u = b * (v - x);
+    float o = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      const f32x4 k = load4(krow + 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g, a.vec_k);
+      const f32x4 q = load4(qrow + 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g, a.vec_q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (16 * dt + 4 * g + i < a.Dk) {
+          S[dt][i] = fmaf(k[i], u, S[dt][i]);
+          o = fmaf(q[i], S[dt][i], o);
+        }
+      }
+    }
+    o = group_sum(o);
+    if (g == 0 && col < a.Dv) {
+      ((T*)a.o)[rows.batch * a.ob + h * a.oh + (row0 + t) * a.on + col] = (T)(a.scale * o);
+      if (SAVE) a.us[((tile * a.H + h) * C + t) * a.Dv + col] = u;
+    }
+  }
+}
+
+template <typename T, int KB, bool SAVE>
+__global__ __launch_bounds__(256) void chain(Args a) {
+  constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>, ORD = kOutOrder<T>;
+  const int64_t seq = blockIdx.x;
+  const int h = blockIdx.y, hk = h / a.group;
+  const int wave = blockIdx.z * (blockDim.x / 64) + threadIdx.x / 64;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  if (16 * wave >= a.Dv) return;
+  const int col = 16 * wave + m;
+  const bool in = col < a.Dv;
+  const Rows rows = rows_of(a.cu, seq, a.N);
+  const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), nch = (rows.n + C - 1) / C;
+  f32x4 S[2 * KB];
+#pragma unroll
+  for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 16 * dt + 4 * g + i;
+      S[dt][i] = a.init && in && d < a.Dk ? a.init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
+    }
+  for (int64_t c = 0; c < nch; ++c) {
+    const int64_t tile = tile0 + c, row0 = rows.first + c * C;
+    const int n = rows.n - c * C < C ? (int)(rows.n - c * C) : C;
+    if (SAVE) {
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 16 * dt + 4 * g + i;
+          if (in && d < a.Dk) a.states[((tile * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+        }
+    }
+    constexpr int kAll = 4 * KB * NI * kFrag;
+    const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
+    const __bf16* tri = tri_tiles<T>(a, tile, h);
+    const float* vec = vec_of(a, tile, h);
+    Terms<NX> s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+    // R
+    f32x4 R[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) x = product<2>(load_terms<NI>(kf + (mt * KB + kb) * NI * kFrag, lane), s[kb], x);
+      const f32x4 bg = *reinterpret_cast<const f32x4*>(vec + V_BG * C + 16 * mt + 4 * g);
+      const f32x4 b = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * mt + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = 16 * mt + 4 * g + i;
+        const float v =
+            t < n && in ? (float)((const T*)a.v)[rows.batch * a.vb + h * a.vh + (row0 + t) * a.vn + col] : 0.f;
+        R[mt][i] = b[i] * v - bg[i] * x[i];
+      }
+    }
+    // U
+    Terms<NX> r[2] = {split<NX>(R[0], R[1]), split<NX>(R[2], R[3])};
+    f32x4 U[4];
+    float odd = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb <= mt / 2; ++kb) x = product<2>(load_terms<NX>(tri + tri_lower(mt, kb) * NX * kFrag, lane), r[kb], x);
+      U[mt] = x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) odd += 0.f * x[i];
+    }
+    // o, transposed: lane m has token 16 mt + m and columns 4g..4g+3 of the wavefront's
+    const Terms<NO> u[2] = {split<NO>(U[0], U[1]), split<NO>(U[2], U[3])};
+    f32x4 O[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        Terms<NO> so;
+#pragma unroll
+        for (int j = 0; j < NO; ++j) so.t[j] = s[kb].t[j];
+        x = product<ORD>(so, load_terms<NI>(kf + 2 * kAll + (mt * KB + kb) * NI * kFrag, lane), x);
+      }
+#pragma unroll
+      for (int kb = 0; kb <= mt / 2; ++kb)
+        y = product<ORD>(u[kb], load_terms<NO>(tri + (kTri * NX + tri_lower(mt, kb) * NO) * kFrag, lane), y);
+      const float since = a.scale * vec[V_SINCE * C + 16 * mt + m];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        O[mt][i] = since * x[i] + y[i];
+        odd += 0.f * O[mt][i];
+      }
+    }
+    if (__any(odd != 0.f)) {  // NaN: something is not finite
+      chunk_by_token<T, KB, SAVE>(a, rows, row0, n, h, col, tile, S);
+      continue;
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const int t = 16 * mt + m;
+      if (t < n)
+        store4((T*)a.o + rows.batch * a.ob + h * a.oh + (row0 + t) * a.on + 16 * wave + 4 * g, O[mt],
+               a.Dv - 16 * wave - 4 * g, a.vec_o);
+    }
+    if (SAVE) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (in) a.us[((tile * a.H + h) * C + 16 * mt + 4 * g + i) * a.Dv + col] = U[mt][i];
+    }
+    // S
+    const float whole = vec[V_SINCE * C + C - 1];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) U[mt] *= *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
+    const Terms<NX> ul[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      S[dt] *= whole;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        S[dt] = product<2>(load_terms<NI>(kf + kAll + (dt * 2 + kb) * NI * kFrag, lane), ul[kb], S[dt]);
+    }
+  }
+  if (a.final) {
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 16 * dt + 4 * g + i;
+        if (in && d < a.Dk) a.final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+      }
+  }
+}
+
+// --------------------------------------------------------------------------
+// Backward.  With dS the gradient of the state at a chunk's end (P with scale):
+//     dU = P' dO + e^{G_64 - G} (K dS)          dR = T' dU
+//     dS <- e^{G_64} dS + scale Q' (e^G dO) - K' (b e^G dR)
+// chain_back() goes through the chunks from the last to the first as chain() does and
+// leaves dR and each chunk's dS; grads() then has everything of its chunk:
+//     dq = scale e^G (S dO) + (dP o D) K           dP_ij = dO_i.u_j,  D_ij = scale e^{G_i - G_j}, j <= i
+//     dk = b rho + kw                              dA_ij = -dR_i.u_j (over b_i: below)
+//     rho_i = -e^{G_i} S dR_i + sum_{j<i} dA_ij e^{G_i-G_j} k_j
+//     kw_j  = e^{G_64-G_j} dS u_j + sum_{i>=j} dP_ij D_ij q_i + sum_{i>j} b_i dA_ij e^{G_i-G_j} k_i
+//     dv = b dR        db_i = dR_i.v_i + k_i.rho_i
+//     dG_i = q_i.dq_i + b_i k_i.rho_i - k_i.kw_i,  and at i = 64 also
+//            e^{G_64} <S, dS> + sum_j e^{G_64-G_j} k_j.(dS u_j)
+//     dg_i = sum of dG_i.. to the chunk's end
+// --------------------------------------------------------------------------
+template <typename T, int KB>
+__global__ __launch_bounds__(256) void chain_back(Args a) {
+  constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>;
+  const int64_t seq = blockIdx.x;
+  const int h = blockIdx.y, hk = h / a.group;
+  const int wave = blockIdx.z * (blockDim.x / 64) + threadIdx.x / 64;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  if (16 * wave >= a.Dv) return;
+  const int col = 16 * wave + m;
+  const bool in = col < a.Dv;
+  const Rows rows = rows_of(a.cu, seq, a.N);
+  const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), nch = (rows.n + C - 1) / C;
+  f32x4 S[2 * KB];
+#pragma unroll
+  for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 16 * dt + 4 * g + i;
+      S[dt][i] = a.d_final && in && d < a.Dk ? a.d_final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
+    }
+  for (int64_t c = nch - 1; c >= 0; --c) {
+    const int64_t tile = tile0 + c, row0 = rows.first + c * C;
+    const int n = rows.n - c * C < C ? (int)(rows.n - c * C) : C;
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 16 * dt + 4 * g + i;
+        if (in && d < a.Dk) a.dstates[((tile * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+      }
+    constexpr int kAll = 4 * KB * NI * kFrag;
+    const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
+    const __bf16* tri = tri_tiles<T>(a, tile, h);
+    const float* vec = vec_of(a, tile, h);
+    f32x4 dO[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = 16 * mt + 4 * g + i;
+        dO[mt][i] =
+            t < n && in ? (float)((const T*)a.d_o)[rows.batch * a.dob + h * a.doh + (row0 + t) * a.don + col] : 0.f;
+      }
+    const Terms<NI> o[2] = {split<NI>(dO[0], dO[1]), split<NI>(dO[2], dO[3])};
+    Terms<NX> s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+    f32x4 U[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) x = product<2>(load_terms<NI>(kf + (mt * KB + kb) * NI * kFrag, lane), s[kb], x);
+      x *= *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
+#pragma unroll
+      for (int kb = mt / 2; kb < 2; ++kb)
+        x = product<2>(load_terms<NO>(tri + (kTri * NX + tri_upper(mt, kb) * NO) * kFrag, lane), o[kb], x);
+      U[mt] = x;
+    }
+    const Terms<NX> u[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
+    f32x4 R[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = mt / 2; kb < 2; ++kb) x = product<2>(load_terms<NX>(tri + tri_upper(mt, kb) * NX * kFrag, lane), u[kb], x);
+      R[mt] = x;
+      const f32x4 b = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * mt + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = 16 * mt + 4 * g + i;
+        if (in) {
+          a.drs[((tile * a.H + h) * C + t) * a.Dv + col] = x[i];
+          if (t < n) ((T*)a.dv)[rows.batch * a.dvb + h * a.dvh + (row0 + t) * a.dvn + col] = (T)(b[i] * x[i]);
+        }
+      }
+    }
+    const float whole = vec[V_SINCE * C + C - 1];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      R[mt] *= *reinterpret_cast<const f32x4*>(vec + V_BG * C + 16 * mt + 4 * g);
+      R[mt] = -R[mt];
+      dO[mt] *= a.scale * *reinterpret_cast<const f32x4*>(vec + V_SINCE * C + 16 * mt + 4 * g);
+    }
+    const Terms<NX> r[2] = {split<NX>(R[0], R[1]), split<NX>(R[2], R[3])};
+    const Terms<NX> e[2] = {split<NX>(dO[0], dO[1]), split<NX>(dO[2], dO[3])};
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      S[dt] *= whole;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        S[dt] = product<2>(load_terms<NI>(kf + kAll + (dt * 2 + kb) * NI * kFrag, lane), r[kb], S[dt]);
+        S[dt] = product<2>(load_terms<NI>(kf + 2 * kAll + (dt * 2 + kb) * NI * kFrag, lane), e[kb], S[dt]);
+      }
+    }
+  }
+  if (a.d_init) {
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 16 * dt + 4 * g + i;
+        if (in && d < a.Dk) a.d_init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+      }
+  }
+}
+
+// Grid (tiles, Hk), four wavefronts; wavefront w has tokens 16w..16w+15, lane m the token
+// 16w + m, and channels 4g.. of each 16-channel tile: no product crosses wavefronts.
+template <typename T, int KB>
+__global__ __launch_bounds__(256) void grads(Args a) {
+  constexpr int NI = kInputTerms<T>;
+  constexpr int kAll = 4 * KB * NI * kFrag;
+  __shared__ float dGs[C], ends[4];
+  const int64_t tile = blockIdx.x;
+  const int hk = blockIdx.y;
+  const int w = threadIdx.x / 64, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  zero_outside<C>(a.cu, a.sequences, tile, a.N, (T*)a.dq + hk * a.dqh, a.dqn, a.Dk, threadIdx.x, 256);
+  zero_outside<C>(a.cu, a.sequences, tile, a.N, (T*)a.dk + hk * a.dkh, a.dkn, a.Dk, threadIdx.x, 256);
+  for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
+    zero_outside<C>(a.cu, a.sequences, tile, a.N, a.dg + h * a.N, 1, 1, threadIdx.x, 256);
+    zero_outside<C>(a.cu, a.sequences, tile, a.N, a.dbeta + h * a.N, 1, 1, threadIdx.x, 256);
+  }
+  const TileOf at = tile_of<C>(a.cu, a.sequences, tile, a.N);
+  const int64_t left_rows = at.rows.n - at.index * C;
+  if (left_rows <= 0) return;
+  const int n = left_rows < C ? (int)left_rows : C;
+  const int64_t row0 = at.rows.first + at.index * C, bt = at.rows.batch;
+  const int t = 16 * w + m;
+  const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
+  f32x4 dq[2 * KB], dk[2 * KB];
+#pragma unroll
+  for (int dt = 0; dt < 2 * KB; ++dt) dq[dt] = dk[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
+    const float* vec = vec_of(a, tile, h);
+    const float* St = a.states + (tile * a.H + h) * (int64_t)a.Dk * a.Dv;
+    const float* dSt = a.dstates + (tile * a.H + h) * (int64_t)a.Dk * a.Dv;
+    const float* Us = a.us + (tile * a.H + h) * (int64_t)C * a.Dv;
+    const float* Rs = a.drs + (tile * a.H + h) * (int64_t)C * a.Dv;
+    const bool vec_f = a.Dv % 4 == 0;
+    f32x4 hq[2 * KB], rho[2 * KB], kw[2 * KB];
+    f32x4 E1[4], E2[4], F1[4], F2[4];  // dO_i.u_j and dR_i.u_j: lane = i, rows j <= i; lane = j, rows i >= j
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) hq[dt] = rho[dt] = kw[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) E1[x] = E2[x] = F1[x] = F2[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float db = 0.f, ss = 0.f;
+    for (int c0 = 0; c0 < a.Dv; c0 += 32) {
+      float xo[8], xr[8], xu[8], xv[8];
+      load8((const T*)a.d_o + bt * a.dob + h * a.doh + (row0 + t) * a.don, c0, g, t < n ? a.Dv : 0, a.vec_do, xo);
+      load8((const T*)a.v + bt * a.vb + h * a.vh + (row0 + t) * a.vn, c0, g, t < n ? a.Dv : 0, a.vec_v, xv);
+      load8(Rs + t * (int64_t)a.Dv, c0, g, t < n ? a.Dv : 0, vec_f, xr);
+      load8(Us + t * (int64_t)a.Dv, c0, g, t < n ? a.Dv : 0, vec_f, xu);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) db = fmaf(xr[i], xv[i], db);
+      const Terms<NI> o = split<NI>(xo);
+      const Terms<NX> r = split<NX>(xr), u = split<NX>(xu);
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt) {
+        const int d = 16 * dt + m;
+        float xs[8], xd[8];
+        load8(St + d * (int64_t)a.Dv, c0, g, d < a.Dk ? a.Dv : 0, vec_f, xs);
+        load8(dSt + d * (int64_t)a.Dv, c0, g, d < a.Dk ? a.Dv : 0, vec_f, xd);
+        if (dt % 4 == w) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss = fmaf(xs[i], xd[i], ss);
+        }
+        const Terms<NX> s = split<NX>(xs), ds = split<NX>(xd);
+        hq[dt] = product<2>(s, o, hq[dt]);
+        rho[dt] = product<2>(s, r, rho[dt]);
+        kw[dt] = product<2>(ds, u, kw[dt]);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int y = 16 * x + m;
+        if (x <= w) {
+          float z[8];
+          load8(Us + y * (int64_t)a.Dv, c0, g, y < n ? a.Dv : 0, vec_f, z);
+          const Terms<NX> uj = split<NX>(z);
+          E1[x] = product<2>(uj, o, E1[x]);
+          E2[x] = product<2>(uj, r, E2[x]);
+        }
+        if (x >= w) {
+          float z[8];
+          load8((const T*)a.d_o + bt * a.dob + h * a.doh + (row0 + y) * a.don, c0, g, y < n ? a.Dv : 0, a.vec_do, z);
+          F1[x] = product<2>(split<NI>(z), u, F1[x]);
+          load8(Rs + y * (int64_t)a.Dv, c0, g, y < n ? a.Dv : 0, vec_f, z);
+          F2[x] = product<2>(split<NX>(z), u, F2[x]);
+        }
+      }
+    }
+    const float Gt = vec[V_G * C + t], Gl = vec[V_GLOW * C + t], bt_ = vec[V_BETA * C + t];
+    const float since = vec[V_SINCE * C + t], left = vec[V_LEFT * C + t], whole = vec[V_SINCE * C + C - 1];
+    // k.(the state's part of kw), q.dq, k.rho, k.kw
+    float kend = 0.f, qq = 0.f, kr = 0.f, kk = 0.f;
+    const T* krow = (const T*)a.k + bt * a.kb + hk * a.kh + (row0 + t) * a.kn;
+    const T* qrow = (const T*)a.q + bt * a.qb + hk * a.qh + (row0 + t) * a.qn;
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      hq[dt] *= a.scale * since;
+      rho[dt] *= -since;
+      kw[dt] *= left;
+      const f32x4 k = load4(krow + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0, a.vec_k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kend = fmaf(k[i], kw[dt][i], kend);
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const f32x4 Gy = *reinterpret_cast<const f32x4*>(vec + V_G * C + 16 * x + 4 * g);
+      const f32x4 Ly = *reinterpret_cast<const f32x4*>(vec + V_GLOW * C + 16 * x + 4 * g);
+      const f32x4 by = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * x + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int y = 16 * x + 4 * g + i;
+        const float d = (Gt - Gy[i]) + (Gl - Ly[i]);
+        const float fi = y <= t ? expf(d) : 0.f, fj = y >= t ? expf(-d) : 0.f;
+        E1[x][i] = y <= t ? a.scale * fi * E1[x][i] : 0.f;
+        E2[x][i] = y < t ? -fi * E2[x][i] : 0.f;
+        F1[x][i] = y >= t ? a.scale * fj * F1[x][i] : 0.f;
+        F2[x][i] = y > t ? -by[i] * fj * F2[x][i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const bool lo = kb <= w / 2, hi = kb >= w / 2;
+      const Terms<NX> e1 = split<NX>(E1[2 * kb], E1[2 * kb + 1]), e2 = split<NX>(E2[2 * kb], E2[2 * kb + 1]);
+      const Terms<NX> f1 = split<NX>(F1[2 * kb], F1[2 * kb + 1]), f2 = split<NX>(F2[2 * kb], F2[2 * kb + 1]);
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt) {
+        const Terms<NI> kT = load_terms<NI>(kf + kAll + (dt * 2 + kb) * NI * kFrag, lane);
+        if (lo) {
+          hq[dt] = product<2>(kT, e1, hq[dt]);
+          rho[dt] = product<2>(kT, e2, rho[dt]);
+        }
+        if (hi) {
+          const Terms<NI> qT = load_terms<NI>(kf + 2 * kAll + (dt * 2 + kb) * NI * kFrag, lane);
+          kw[dt] = product<2>(qT, f1, kw[dt]);
+          kw[dt] = product<2>(kT, f2, kw[dt]);
+        }
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      const f32x4 k = load4(krow + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0, a.vec_k);
+      const f32x4 q = load4(qrow + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0, a.vec_q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qq = fmaf(q[i], hq[dt][i], qq);
+        kr = fmaf(k[i], rho[dt][i], kr);
+        kk = fmaf(k[i], kw[dt][i], kk);
+        dq[dt][i] += hq[dt][i];
+        dk[dt][i] += fmaf(bt_, rho[dt][i], kw[dt][i]);
+      }
+    }
+    kend = group_sum(kend), qq = group_sum(qq), kr = group_sum(kr), kk = group_sum(kk), db = group_sum(db);
+    // Over the tokens (kend) and channels (ss) of this wavefront.
+#pragma unroll
+    for (int x = 1; x < 16; x *= 2) {
+      kend += __shfl_xor(kend, x);
+      ss += __shfl_xor(ss, x);
+    }
+    ss = group_sum(ss);
+    __syncthreads();  // dGs and ends of the head before are read
+    if (g == 0) {
+      dGs[t] = qq + bt_ * kr - kk;
+      if (t < n) a.dbeta[(bt * a.H + h) * a.N + row0 + t] = db + kr;
+    }
+    if (lane == 0) ends[w] = kend + whole * ss;
+    __syncthreads();
+    if (w == 0) {
+      float x = dGs[lane];
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const float y = __shfl_down(x, d);
+        if (lane + d < 64) x += y;
+      }
+      if (lane < n) a.dg[(bt * a.H + h) * a.N + row0 + lane] = x + ((ends[0] + ends[1]) + (ends[2] + ends[3]));
+    }
+  }
+  if (t < n) {
+    T* dqrow = (T*)a.dq + bt * a.dqb + hk * a.dqh + (row0 + t) * a.dqn;
+    T* dkrow = (T*)a.dk + bt * a.dkb + hk * a.dkh + (row0 + t) * a.dkn;
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      store4(dqrow + 16 * dt + 4 * g, dq[dt], a.Dk - 16 * dt - 4 * g, a.vec_dq);
+      store4(dkrow + 16 * dt + 4 * g, dk[dt], a.Dk - 16 * dt - 4 * g, a.vec_dk);
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
+// One token.  Bound by the state, read and written once: a workgroup has 32
+// columns of one head's state, in registers between the two.
+//     x = k'S, y = q'S;  u = b (v - a x);  S <- a S + k u';  o = scale (a y + (q.k) u)
+// --------------------------------------------------------------------------
+constexpr int kStepCols = 32;
+
+template <typename T, typename TO>
+__global__ __launch_bounds__(256) void step(const T* q, const T* k, const T* v, const float* gs, const float* betas,
+                                            const float* in, float* out_state, TO* out, int Hk, int H, int Dk, int Dv,
+                                            float scale, bool vec_in, bool vec_out) {
+  // Eight lanes of four columns; 32 rows at a time.
+  __shared__ float xs[4][kStepCols], ys[4][kStepCols], dots[4];
+  const int64_t bh = blockIdx.x;
+  const int64_t b = bh / H, h = bh % H;
+  const T* kp = k + (b * Hk + h / (H / Hk)) * Dk;
+  const T* qp = q + (b * Hk + h / (H / Hk)) * Dk;
+  const int c = blockIdx.y * kStepCols + (threadIdx.x & 7) * 4, r0 = threadIdx.x >> 3, w = threadIdx.x >> 6;
+  const float dec = expf(gs[bh]), beta = betas[bh];
+  constexpr int R = KDELTA_MAX_DK / 32;
+  f32x4 S[R];
+  float kk[R], qk = 0.f;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int r = r0 + 32 * j;
+    const bool on = r < Dk;
+    S[j] = load4(in + (bh * Dk + (on ? r : 0)) * (int64_t)Dv + c, on ? Dv - c : 0, vec_in);
+    kk[j] = on ? (float)kp[r] : 0.f;
+    const float qq = on ? (float)qp[r] : 0.f;
+    qk = fmaf(kk[j], qq, qk);
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        S[j][i] *= dec;
+        x[i] = fmaf(kk[j], S[j][i], x[i]);
+        y[i] = fmaf(qq, S[j][i], y[i]);
+      }
+    }
+  }
+  // over the rows: lanes 8 apart, then the four wavefronts
+#pragma unroll
+  for (int d = 8; d < 64; d *= 2) {
+    qk += __shfl_xor(qk, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] += __shfl_xor(x[i], d);
+      y[i] += __shfl_xor(y[i], d);
+    }
+  }
+  if ((threadIdx.x & 63) < 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      xs[w][(threadIdx.x & 7) * 4 + i] = x[i];
+      ys[w][(threadIdx.x & 7) * 4 + i] = y[i];
+    }
+    if ((threadIdx.x & 7) == 0) dots[w] = qk;
+  }
+  __syncthreads();
+  qk = (dots[0] + dots[1]) + (dots[2] + dots[3]);
+  const f32x4 vv = load4(v + bh * Dv + c, Dv - c, false);
+  f32x4 u, o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int cc = (threadIdx.x & 7) * 4 + i;
+    const float xx = (xs[0][cc] + xs[1][cc]) + (xs[2][cc] + xs[3][cc]);
+    const float yy = (ys[0][cc] + ys[1][cc]) + (ys[2][cc] + ys[3][cc]);
+    u[i] = beta * (vv[i] - xx);
+    o[i] = scale * (yy + qk * u[i]);
+  }
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int r = r0 + 32 * j;
+    if (r >= Dk) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) S[j][i] = fmaf(kk[j], u[i], S[j][i]);
+    store4(out_state + (bh * Dk + r) * (int64_t)Dv + c, S[j], Dv - c, vec_out);
+  }
+  if (threadIdx.x < 8) store4(out + bh * Dv + c, o, Dv - c, false);
+}
+
+// --------------------------------------------------------------------------
+// Host
+// --------------------------------------------------------------------------
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+int64_t tiles_of(const kdelta_problem* p) {
+  return p->cu_seqlens ? p->N / C + p->sequences : p->B * ((p->N + C - 1) / C);
+}
+
+int input_terms(int dtype) { return dtype == KDECAY_BF16 ? 1 : dtype == KDECAY_F16 ? 2 : 3; }
+
+struct Sizes {
+  size_t keys, tris, vecs, dstates, drs;
+};
+
+Sizes sizes_of(const kdelta_problem* p) {
+  const size_t tiles = tiles_of(p), KB = (p->Dk + 31) / 32, NI = input_terms(p->dtype);
+  const size_t NO = p->dtype == KDECAY_F32 ? 3 : 2;
+  Sizes s;
+  s.keys = up256(tiles * p->Hk * 3 * 4 * KB * NI * kFrag * 2);
+  s.tris = up256(tiles * p->H * kTri * (NX + NO) * kFrag * 2);
+  s.vecs = up256(tiles * p->H * V_COUNT * C * 4);
+  s.dstates = up256(tiles * p->H * p->Dk * p->Dv * 4);
+  s.drs = up256(tiles * p->H * C * p->Dv * 4);
+  return s;
+}
+
+bool aligned4(const void* p, const int64_t* st, int dtype) {
+  return ((uintptr_t)p & (dtype == KDECAY_F32 ? 15u : 7u)) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+}
+
+int check(const kdelta_problem* p) {
+  if (!p) return fail(KDECAY_EINVAL, "null problem");
+  if (p->B < 0 || p->Hk < 0 || p->H < 0 || p->N < 0 || p->Dk < 0 || p->Dv < 0 || p->sequences < 0)
+    return fail(KDECAY_EINVAL, "negative size");
+  if (p->dtype != KDECAY_F32 && p->dtype != KDECAY_BF16 && p->dtype != KDECAY_F16)
+    return fail(KDECAY_EDTYPE, "q, k and v must be float32, bfloat16 or float16 (code %d)", p->dtype);
+  if (p->Dk < 1 || p->Dk > KDELTA_MAX_DK || p->Dv < 1 || p->Dv > KDELTA_MAX_DV)
+    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not 1..%d and 1..%d", (long long)p->Dk,
+                (long long)p->Dv, KDELTA_MAX_DK, KDELTA_MAX_DV);
+  if (p->Hk < 1 || p->H < 1 || p->H % p->Hk) return fail(KDECAY_ESHAPE, "H=%lld is no multiple of Hk=%lld", (long long)p->H, (long long)p->Hk);
+  if (p->H > 65535) return fail(KDECAY_ESHAPE, "more than 65535 heads");
+  if (p->cu_seqlens && (p->B != 1 || p->sequences < 1))
+    return fail(KDECAY_ESHAPE, "cu_seqlens takes B=1 and at least one sequence");
+  if (!p->cu_seqlens && p->sequences != p->B) return fail(KDECAY_EINVAL, "sequences must be B without cu_seqlens");
+  if (p->sequences > 0x7fffffff || tiles_of(p) > 0x7fffffff) return fail(KDECAY_ESHAPE, "too many sequences or rows");
+  if (p->B && p->N && (!p->q || !p->k || !p->v || !p->g || !p->beta)) return fail(KDECAY_EINVAL, "null pointer argument");
+  if ((p->q_strides[3] != 1 && p->Dk != 1) || (p->k_strides[3] != 1 && p->Dk != 1) || (p->v_strides[3] != 1 && p->Dv != 1))
+    return fail(KDECAY_ELAYOUT, "channel (d) stride must be 1");
+  return 0;
+}
+
+Args args_of(const kdelta_problem* p, void* workspace) {
+  Args a = {};
+  a.q = p->q, a.k = p->k, a.v = p->v, a.g = p->g, a.beta = p->beta, a.cu = p->cu_seqlens, a.init = p->init;
+  a.qb = p->q_strides[0], a.qh = p->q_strides[1], a.qn = p->q_strides[2];
+  a.kb = p->k_strides[0], a.kh = p->k_strides[1], a.kn = p->k_strides[2];
+  a.vb = p->v_strides[0], a.vh = p->v_strides[1], a.vn = p->v_strides[2];
+  a.gb = p->g_strides[0], a.gh = p->g_strides[1], a.gn = p->g_strides[2];
+  a.bb = p->beta_strides[0], a.bh = p->beta_strides[1], a.bn = p->beta_strides[2];
+  a.N = p->N, a.sequences = p->sequences, a.tiles = tiles_of(p);
+  a.Hk = (int)p->Hk, a.H = (int)p->H, a.Dk = (int)p->Dk, a.Dv = (int)p->Dv, a.group = (int)(p->H / p->Hk);
+  a.scale = p->scale;
+  a.vec_q = aligned4(p->q, p->q_strides, p->dtype);
+  a.vec_k = aligned4(p->k, p->k_strides, p->dtype);
+  a.vec_v = aligned4(p->v, p->v_strides, p->dtype);
+  const Sizes s = sizes_of(p);
+  char* w = (char*)workspace;
+  a.keys = (__bf16*)w;
+  a.tris = (__bf16*)(w + s.keys);
+  a.vecs = (float*)(w + s.keys + s.tris);
+  a.dstates = (float*)(w + s.keys + s.tris + s.vecs);
+  a.drs = (float*)(w + s.keys + s.tris + s.vecs + s.dstates);
+  return a;
+}
+
+template <typename F>
+int by_type(int dtype, F f) {
+  if (dtype == KDECAY_BF16) return f((__bf16*)nullptr);
+  if (dtype == KDECAY_F16) return f((_Float16*)nullptr);
+  return f((float*)nullptr);
+}
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+template <typename F>
+int by_blocks(int64_t Dk, F f) {
+  switch ((Dk + 31) / 32) {
+    case 1: return f(Int<1>());
+    case 2: return f(Int<2>());
+    case 3: return f(Int<3>());
+    default: return f(Int<4>());
+  }
+}
+
+// Wavefronts of one workgroup of chain() and chain_back(), each with 16 columns.
+constexpr int kChainWaves = 4;
+dim3 chain_grid(const Args& a) {
+  const int waves = (a.Dv + 15) / 16;
+  return dim3((unsigned)a.sequences, a.H, (waves + kChainWaves - 1) / kChainWaves);
+}
+
+}  // namespace delta
+}  // namespace kd
+
+using namespace kd;
+using namespace kd::delta;
+
+extern "C" size_t kdelta_scan_workspace_bytes(const kdelta_problem* p) {
+  if (check(p)) return 0;
+  const Sizes s = sizes_of(p);
+  return s.keys + s.tris + s.vecs;
+}
+
+extern "C" size_t kdelta_scan_bwd_workspace_bytes(const kdelta_problem* p) {
+  if (check(p)) return 0;
+  const Sizes s = sizes_of(p);
+  return s.keys + s.tris + s.vecs + s.dstates + s.drs;
+}
+
+extern "C" size_t kdelta_scan_saved_floats(const kdelta_problem* p) {
+  if (check(p)) return 0;
+  return (size_t)tiles_of(p) * p->H * (p->Dk + C) * p->Dv;
+}
+
+extern "C" int kdelta_scan_fwd(const kdelta_problem* p, void* o, const int64_t* o_strides, float* final, float* saved,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check(p)) return rc;
+  if (p->sequences == 0) return 0;
+  const bool rows = p->B && p->N;
+  if (rows && (!o || !o_strides)) return fail(KDECAY_EINVAL, "null pointer argument");
+  if (rows && o_strides[3] != 1 && p->Dv != 1) return fail(KDECAY_ELAYOUT, "channel (d) stride must be 1");
+  if (workspace_bytes < kdelta_scan_workspace_bytes(p) || (!workspace && rows) || ((uintptr_t)workspace & 15))
+    return fail(KDECAY_EWORKSPACE, "scan workspace of %zu bytes missing, small or not 16-byte aligned",
+                kdelta_scan_workspace_bytes(p));
+  if ((uintptr_t)saved & 15) return fail(KDECAY_ELAYOUT, "saved is not 16-byte aligned");
+  Args a = args_of(p, workspace);
+  a.o = o, a.final = final;
+  if (rows) a.ob = o_strides[0], a.oh = o_strides[1], a.on = o_strides[2], a.vec_o = aligned4(o, o_strides, p->dtype);
+  a.states = saved;
+  a.us = saved ? saved + (size_t)a.tiles * a.H * a.Dk * a.Dv : nullptr;
+  const hipStream_t s = (hipStream_t)stream;
+  return by_type(p->dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return by_blocks(p->Dk, [&](auto kb) {
+      constexpr int KB = decltype(kb)::value;
+      if (rows) {
+        prep<T, KB, false><<<dim3((unsigned)a.tiles, a.H), 256, 0, s>>>(a);
+        if (const int rc = hip_check("kdelta prep launch")) return rc;
+      }
+      if (saved)
+        chain<T, KB, true><<<chain_grid(a), 64 * kChainWaves, 0, s>>>(a);
+      else
+        chain<T, KB, false><<<chain_grid(a), 64 * kChainWaves, 0, s>>>(a);
+      return hip_check("kdelta chain launch");
+    });
+  });
+}
+
+extern "C" int kdelta_scan_bwd(const kdelta_problem* p, const void* d_o, const int64_t* do_strides,
+                               const float* d_final, const float* saved, void* dq, const int64_t* dq_strides, void* dk,
+                               const int64_t* dk_strides, void* dv, const int64_t* dv_strides, float* dg, float* dbeta,
+                               float* d_init, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check(p)) return rc;
+  if (p->sequences == 0) return 0;
+  const bool rows = p->B && p->N;
+  if (rows && (!d_o || !do_strides || !saved || !dq || !dq_strides || !dk || !dk_strides || !dv || !dv_strides || !dg || !dbeta))
+    return fail(KDECAY_EINVAL, "null pointer argument");
+  if (rows && ((do_strides[3] != 1 && p->Dv != 1) || (dq_strides[3] != 1 && p->Dk != 1) ||
+               (dk_strides[3] != 1 && p->Dk != 1) || (dv_strides[3] != 1 && p->Dv != 1)))
+    return fail(KDECAY_ELAYOUT, "channel (d) stride must be 1");
+  if (workspace_bytes < kdelta_scan_bwd_workspace_bytes(p) || (!workspace && rows) || ((uintptr_t)workspace & 15))
+    return fail(KDECAY_EWORKSPACE, "backward workspace of %zu bytes missing, small or not 16-byte aligned",
+                kdelta_scan_bwd_workspace_bytes(p));
+  if ((uintptr_t)saved & 15) return fail(KDECAY_ELAYOUT, "saved is not 16-byte aligned");
+  Args a = args_of(p, workspace);
+  a.states = const_cast<float*>(saved);
+  a.us = a.states + (size_t)a.tiles * a.H * a.Dk * a.Dv;
+  a.d_o = d_o, a.d_final = d_final, a.d_init = d_init, a.dq = dq, a.dk = dk, a.dv = dv, a.dg = dg, a.dbeta = dbeta;
+  if (rows) {
+    a.dob = do_strides[0], a.doh = do_strides[1], a.don = do_strides[2];
+    a.dqb = dq_strides[0], a.dqh = dq_strides[1], a.dqn = dq_strides[2];
+    a.dkb = dk_strides[0], a.dkh = dk_strides[1], a.dkn = dk_strides[2];
+    a.dvb = dv_strides[0], a.dvh = dv_strides[1], a.dvn = dv_strides[2];
+    a.vec_do = aligned4(d_o, do_strides, p->dtype);
+    a.vec_dq = aligned4(dq, dq_strides, p->dtype);
+    a.vec_dk = aligned4(dk, dk_strides, p->dtype);
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  return by_type(p->dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return by_blocks(p->Dk, [&](auto kb) {
+      constexpr int KB = decltype(kb)::value;
+      if (rows) {
+        prep<T, KB, true><<<dim3((unsigned)a.tiles, a.H), 256, 0, s>>>(a);
+        if (const int rc = hip_check("kdelta prep launch")) return rc;
+      }
+      chain_back<T, KB><<<chain_grid(a), 64 * kChainWaves, 0, s>>>(a);
+      if (const int rc = hip_check("kdelta chain_back launch")) return rc;
+      if (!rows) return 0;
+      grads<T, KB><<<dim3((unsigned)a.tiles, a.Hk), 256, 0, s>>>(a);
+      return hip_check("kdelta grads launch");
+    });
+  });
+}
+
+extern "C" int kdelta_step(const void* q, const void* k, const void* v, int dtype, const float* g, const float* beta,
+                           const float* state_in, float* state_out, void* out, int out_dtype, int64_t B, int64_t Hk,
+                           int64_t H, int64_t Dk, int64_t Dv, float scale, void* stream) {
+  if (B < 0 || Hk < 0 || H < 0 || Dk < 0 || Dv < 0) return fail(KDECAY_EINVAL, "negative size");
+  if (dtype != KDECAY_F32 && dtype != KDECAY_BF16 && dtype != KDECAY_F16)
+    return fail(KDECAY_EDTYPE, "q, k and v must be float32, bfloat16 or float16 (code %d)", dtype);
+  if (out_dtype != dtype && out_dtype != KDECAY_F32) return fail(KDECAY_EDTYPE, "out must have v's type or float32");
+  if (Dk < 1 || Dk > KDELTA_MAX_DK || Dv < 1 || Dv > KDELTA_MAX_DV)
+    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not 1..%d and 1..%d", (long long)Dk, (long long)Dv,
+                KDELTA_MAX_DK, KDELTA_MAX_DV);
+  if (Hk < 1 || H < 1 || H % Hk) return fail(KDECAY_ESHAPE, "H=%lld is no multiple of Hk=%lld", (long long)H, (long long)Hk);
+  if (B == 0) return 0;
+  if (B * H > 0x7fffffff) return fail(KDECAY_ESHAPE, "too many heads");
+  if (!q || !k || !v || !g || !beta || !state_in || !state_out || !out) return fail(KDECAY_EINVAL, "null pointer argument");
+  const bool vec_in = Dv % 4 == 0 && ((uintptr_t)state_in & 15) == 0, vec_out = Dv % 4 == 0 && ((uintptr_t)state_out & 15) == 0;
+  const dim3 grid((unsigned)(B * H), (unsigned)((Dv + kStepCols - 1) / kStepCols));
+  return by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (out_dtype == dtype)
+      step<T, T><<<grid, 256, 0, (hipStream_t)stream>>>((const T*)q, (const T*)k, (const T*)v, g, beta, state_in,
+                                                        state_out, (T*)out, (int)Hk, (int)H, (int)Dk, (int)Dv, scale, vec_in, vec_out);
+    else
+      step<T, float><<<grid, 256, 0, (hipStream_t)stream>>>((const T*)q, (const T*)k, (const T*)v, g, beta, state_in,
+                                                            state_out, (float*)out, (int)Hk, (int)H, (int)Dk, (int)Dv,
+                                                            scale, vec_in, vec_out);
+    return hip_check("kdelta_step launch");
+  });
+}

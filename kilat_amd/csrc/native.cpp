@@ -458,6 +458,8 @@ py::object decay_step(const py::object& lam_o, const py::object& state_o, const 
 
 }  // namespace
 
+void bind_mixers(py::module_& m);  // native_mixers.cpp
+
 PYBIND11_MODULE(_native, m) {
   m.doc() = "Host path of kilat_amd (see native.cpp).";
   m.def("scan", &scan);
@@ -472,4 +474,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("vector_layout_ok", &vector_layout_ok);
   m.def("bwd_rows_fit", &bwd_rows_fit);
   m.def("narrow_rows", &narrow_rows, py::arg("V"), py::arg("train") = false, py::arg("wide") = false);
+  bind_mixers(m);
 }
