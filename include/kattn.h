@@ -25,8 +25,9 @@ extern "C" {
 #define KATTN_MAX_DV 128
 
 /*
- * q [B,H,N,Dk], k [B,Hk,N,Dk], v [B,Hk,N,Dv], with strides for their four dimensions; the
- * last stride is 1 unless the head dim is 1.  cu_seqlens and sequences: as in
+ * q [B,H,N,Dk], k [B,Hk,N,Dk], v [B,Hk,N,Dv], with strides for their four dimensions, as
+ * kdelta.h asks of rows: the last is 1, the others, the bases and the head dims multiples of
+ * four elements.  cu_seqlens and sequences: as in
  * kdelta.h (kdelta_problem).
  */
 typedef struct kattn_problem {

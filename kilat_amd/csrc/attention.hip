@@ -95,13 +95,12 @@ struct Args {
   int64_t N, sequences, tiles;
   int H, Dk, Dv, group;
   float scale;
-  bool vec_q, vec_k, vec_v, vec_o;  // rows start on four elements
 };
 
-// Element values p[0..7], zero from n on.
+// Eight elements from base + at, n of them there.
 template <typename T>
-__device__ __forceinline__ void load_row8(const T* p, int n, bool vec, float (&x)[8]) {
-  const f32x4 a = load4(p, n, vec), b = load4(p + 4, n - 4, vec);
+__device__ __forceinline__ void load_row8(const T* base, int64_t at, int n, float (&x)[8]) {
+  const f32x4 a = load4(base, at, n), b = load4(base, at + 4, n - 4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
 }
@@ -130,11 +129,11 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
   const bool live = row < at.rows.n;
   Operand<T> q[KS];
   {
-    const T* p = (const T*)a.q + at.rows.batch * a.qb + h * a.qh + (at.rows.first + row) * a.qn;
+    const T* p = (const T*)a.q + at.rows.batch * a.qb + h * a.qh + at.rows.first * a.qn;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       float x[8];
-      load_row8(p + 16 * s + 8 * half, live ? a.Dk - 16 * s - 8 * half : 0, a.vec_q, x);
+      load_row8(p, row * a.qn + 16 * s + 8 * half, live ? a.Dk - 16 * s - 8 * half : 0, x);
       q[s] = to_operand<T>(x);
     }
   }
@@ -154,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
     for (int i = tid; i < BK * 2 * KS; i += kThreads) {
       const int key = i / (2 * KS), c = i % (2 * KS);
       float x[8];
-      load_row8(kp + (k0 + key) * a.kn + 8 * c, k0 + key < at.rows.n ? a.Dk - 8 * c : 0, a.vec_k, x);
+      load_row8(kp, (k0 + key) * a.kn + 8 * c, k0 + key < at.rows.n ? a.Dk - 8 * c : 0, x);
       const Operand<T> y = to_operand<T>(x);
       const int slot = ((key & 31) + 32 * (c & 1)) ^ (c & 15);
 #pragma unroll
@@ -169,7 +168,7 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t key = k0 + 4 * kg + j;
-        x[j] = load4(vp + key * a.vn + c, key < at.rows.n ? a.Dv - c : 0, a.vec_v);
+        x[j] = load4(vp, key * a.vn + c, key < at.rows.n ? a.Dv - c : 0);
         if (masked) {
 #pragma unroll
           for (int d = 0; d < 4; ++d)
@@ -280,12 +279,8 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
     for (int r = 0; r < 16; r += 4) {
       const int c = 32 * vt + 2 * r + 4 * half;
       const f32x4 x = {O[vt][r] / l, O[vt][r + 1] / l, O[vt][r + 2] / l, O[vt][r + 3] / l};
-      store4(p + c, x, a.Dv - c, a.vec_o);
+      if (c < a.Dv) store4(p + c, x);
     }
-}
-
-bool aligned4(const void* p, const int64_t* st, int dtype) {
-  return ((uintptr_t)p & (dtype == KDECAY_F32 ? 15u : 7u)) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
 }
 
 template <int BLOCK>
@@ -293,7 +288,7 @@ int64_t tiles_of(const kattn_problem* p) {
   return p->cu_seqlens ? p->N / BLOCK + p->sequences : p->B * ((p->N + BLOCK - 1) / BLOCK);
 }
 
-int check(const kattn_problem* p, const int64_t* o_strides) {
+int check(const kattn_problem* p, const void* o, const int64_t* o_strides) {
   if (!p) return fail(KDECAY_EINVAL, "null problem");
   if (p->B < 0 || p->Hk < 0 || p->H < 0 || p->N < 0 || p->Dk < 0 || p->Dv < 0 || p->sequences < 0)
     return fail(KDECAY_EINVAL, "negative size");
@@ -310,11 +305,14 @@ int check(const kattn_problem* p, const int64_t* o_strides) {
   if (!p->cu_seqlens && p->sequences != p->B) return fail(KDECAY_EINVAL, "sequences must be B without cu_seqlens");
   if (p->sequences > 0x7fffffff || tiles_of<32>(p) > 0x7fffffff)
     return fail(KDECAY_ESHAPE, "too many sequences or rows");
+  if (p->Dk % 4 || p->Dv % 4)
+    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not multiples of 4", (long long)p->Dk, (long long)p->Dv);
   if (!p->B || !p->N) return 0;
-  if (!p->q || !p->k || !p->v || !o_strides) return fail(KDECAY_EINVAL, "null pointer argument");
-  if (((p->q_strides[3] != 1 || p->k_strides[3] != 1) && p->Dk != 1) ||
-      ((p->v_strides[3] != 1 || o_strides[3] != 1) && p->Dv != 1))
-    return fail(KDECAY_ELAYOUT, "channel (d) stride must be 1");
+  if (!p->q || !p->k || !p->v || !o || !o_strides) return fail(KDECAY_EINVAL, "null pointer argument");
+  if (const int rc = check_rows(p->q, p->q_strides, p->dtype, "q")) return rc;
+  if (const int rc = check_rows(p->k, p->k_strides, p->dtype, "k")) return rc;
+  if (const int rc = check_rows(p->v, p->v_strides, p->dtype, "v")) return rc;
+  if (const int rc = check_rows(o, o_strides, p->dtype, "o")) return rc;
   return 0;
 }
 
@@ -325,9 +323,8 @@ using namespace kd;
 using namespace kd::attn;
 
 extern "C" int kattn_fwd(const kattn_problem* p, void* o, const int64_t* o_strides, void* stream) {
-  if (const int rc = check(p, o_strides)) return rc;
+  if (const int rc = check(p, o, o_strides)) return rc;
   if (!p->B || !p->N) return 0;
-  if (!o) return fail(KDECAY_EINVAL, "null pointer argument");
   Args a = {};
   a.q = p->q, a.k = p->k, a.v = p->v, a.o = o, a.cu = p->cu_seqlens;
   a.qb = p->q_strides[0], a.qh = p->q_strides[1], a.qn = p->q_strides[2];
@@ -337,10 +334,6 @@ extern "C" int kattn_fwd(const kattn_problem* p, void* o, const int64_t* o_strid
   a.N = p->N, a.sequences = p->sequences, a.tiles = tiles_of<BQ>(p);
   a.H = (int)p->H, a.Dk = (int)p->Dk, a.Dv = (int)p->Dv, a.group = (int)(p->H / p->Hk);
   a.scale = p->scale;
-  a.vec_q = aligned4(p->q, p->q_strides, p->dtype);
-  a.vec_k = aligned4(p->k, p->k_strides, p->dtype);
-  a.vec_v = aligned4(p->v, p->v_strides, p->dtype);
-  a.vec_o = aligned4(o, o_strides, p->dtype);
   const auto launch = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const dim3 grid((unsigned)a.tiles, a.H);

@@ -44,30 +44,27 @@ struct Args {
   const float* init;
   int64_t qb, qh, qn, kb, kh, kn, vb, vh, vn, gb, gh, gn, bb, bh, bn;
   int64_t N, sequences, tiles;
-  int Hk, H, Dk, Dv, group;
+  int Hk, H, Dk, Dv, group, groups;  // value heads of a key head; 16-column groups of Dv
   float scale;
-  bool vec_k, vec_q, vec_v;  // rows start on four elements
   // scratch, by tile and head
-  __bf16* keys;    // [tiles][Hk][3][4 KB][NI][kFrag]: K, its transpose, Q (backward: its transpose)
-  __bf16* tris;    // [tiles][H][kTri * (NX + kOutTerms)][kFrag]: T and P (backward: transposed)
+  float* inv;      // [tiles][H][kTri][2][64][4]: T as operand tiles
+  __bf16* keys;    // backward: [tiles][Hk][3][4 KB][NI][kFrag]: K, its transpose, Q's transpose
+  __bf16* tris;    // backward: [tiles][H][kTri * 2 * NX][kFrag]: T's transpose and P's
   float* vecs;     // [tiles][H][V_COUNT][C]
-  float* states;   // saved: [tiles][H][Dk][Dv], S at the chunk's start
-  float* us;       // saved: [tiles][H][C][Dv]
+  float* states;   // saved: [tiles][H][16-column groups][2 KB][64][4], S at the chunk's start as it lies in registers
+  float* us;       // saved: [tiles][H][16-column groups][4][64][4]: u
   void* o;
   int64_t ob, oh, on;
-  bool vec_o;
   float* final;
   // backward
   const void* d_o;
   int64_t dob, doh, don;
-  bool vec_do;
   const float* d_final;
   float* d_init;
   float* dstates;  // [tiles][H][Dk][Dv], the gradient of the state at the chunk's end
   float* drs;      // [tiles][H][C][Dv], the gradient of R
   void *dq, *dk, *dv;
   int64_t dqb, dqh, dqn, dkb, dkh, dkn, dvb, dvh, dvn;
-  bool vec_dq, vec_dk;
   float *dg, *dbeta;
 };
 
@@ -76,9 +73,8 @@ template <int KB, int NI>
 __device__ __forceinline__ __bf16* key_tiles(const Args& a, int64_t tile, int hk) {
   return a.keys + ((tile * a.Hk + hk) * 3) * (int64_t)(4 * KB * NI * kFrag);
 }
-template <typename T>
 __device__ __forceinline__ __bf16* tri_tiles(const Args& a, int64_t tile, int h) {
-  return a.tris + (tile * a.H + h) * (int64_t)(kTri * (NX + kOutTerms<T>)*kFrag);
+  return a.tris + (tile * a.H + h) * (int64_t)(kTri * 2 * NX * kFrag);
 }
 __device__ __forceinline__ float* vec_of(const Args& a, int64_t tile, int h) {
   return a.vecs + (tile * a.H + h) * (int64_t)(V_COUNT * C);
@@ -97,6 +93,30 @@ __device__ __forceinline__ void store_terms(__bf16* p, int lane, const Terms<N>&
   for (int n = 0; n < N; ++n) *reinterpret_cast<bf16x8*>(p + n * kFrag + lane * 8) = x.t[n];
 }
 
+// Tile f of the transpose of a chunk's rows, from their tiles in LDS (rows are channels
+// 16 (f / 2) + lane % 16, inner indices tokens of half f % 2).
+template <int KB, int NI>
+__device__ __forceinline__ Terms<NI> transposed(const __bf16* tiles, int f, int lane) {
+  const int d = 16 * (f / 2) + (lane & 15), t0 = 32 * (f & 1) + 4 * (lane >> 4);
+  const int src = (d / 32) * NI * kFrag + (d & 3) + ((d >> 4) & 1) * 4, sl = 16 * ((d >> 2) & 3);
+  Terms<NI> r;
+#pragma unroll
+  for (int j = 0; j < NI; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = t0 + (i & 3) + 16 * (i >> 2);
+      r.t[j][i] = tiles[(t >> 4) * KB * NI * kFrag + src + j * kFrag + (sl + (t & 15)) * 8];
+    }
+  return r;
+}
+
+// A barrier that orders LDS accesses only: loads from global memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // e^x for a difference of sums of log decays (positive for a growing state only).
 __device__ __forceinline__ float fade(double x) {
   const float hi = (float)x, e = expf(hi);
@@ -104,25 +124,26 @@ __device__ __forceinline__ float fade(double x) {
 }
 
 // --------------------------------------------------------------------------
-// prep: T, P and the operand tiles of one chunk and value head
+// prep: T of one chunk and value head (BWD: what the backward's products take)
 // --------------------------------------------------------------------------
 // Grid (tiles, H), four wavefronts; wavefront w has tokens 16w..16w+15 of the chunk.
-// BWD: T, P and Q transposed, as the backward reads them.
+// Forward: T, as operand tiles in 32 bits.  BWD: T and P transposed, K, K transposed and
+// Q transposed, as operand tiles of terms.
 //
 // log decays are added up in 64 bits: the sums over a chunk can be far larger than
 // the differences that count.  One below -128 is taken as -128: e^-128 is 0 in 32 bits,
 // and no difference becomes inf - inf.
 template <typename T, int KB, bool BWD>
 __global__ __launch_bounds__(256) void prep(Args a) {
-  constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>;
+  constexpr int NI = kInputTerms<T>;
   constexpr int LD = C + 4;
-  __shared__ __bf16 kq[2][4 * KB * NI * kFrag];  // K and Q
+  __shared__ __bf16 kq[BWD ? 2 : 1][4 * KB * NI * kFrag];  // K and Q
   __shared__ float As[C * LD], Ts[C * LD];
   __shared__ double Gs[C];
   __shared__ float bs[C];
   const int64_t tile = blockIdx.x;
   const int h = blockIdx.y, hk = h / a.group;
-  const int w = threadIdx.x / 64, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int w = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   if (!BWD)
     zero_outside<C>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, threadIdx.x, 256);
   else
@@ -132,6 +153,19 @@ __global__ __launch_bounds__(256) void prep(Args a) {
   if (left_rows <= 0) return;
   const int n = left_rows < C ? (int)left_rows : C;
   const int64_t row0 = at.rows.first + at.index * C;
+  // Operand tiles of K (and Q): lane (m, g) has token 16w + m.
+  const int t = 16 * w + m;
+  const T* kbase = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + row0 * a.kn;
+  const T* qbase = (const T*)a.q + at.rows.batch * a.qb + hk * a.qh + row0 * a.qn;
+  Raw4<T> kr[KB][2], qr[BWD ? KB : 1][2];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int d = 32 * kb + 16 * x + 4 * g, left = t < n ? a.Dk - d : 0;
+      kr[kb][x] = fetch4(kbase, t * a.kn + d, left);
+      if (BWD) qr[BWD ? kb : 0][x] = fetch4(qbase, t * a.qn + d, left);
+    }
   if (w == 0) {
     const bool in = lane < n;
     double G = 0.;
@@ -158,57 +192,37 @@ __global__ __launch_bounds__(256) void prep(Args a) {
     vec[V_G * C + lane] = (float)G;
     vec[V_GLOW * C + lane] = (float)(G - (double)(float)G);
   }
-  // Operand tiles of K and Q: lane (m, g) has token 16w + m.
-  const int t = 16 * w + m;
-  const T* krow = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + (row0 + t) * a.kn;
-  const T* qrow = (const T*)a.q + at.rows.batch * a.qb + hk * a.qh + (row0 + t) * a.qn;
-  Terms<NI> kt[KB], qt[KB];
+  Terms<NI> kt[KB];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    float x[8];
-    load8(krow, 32 * kb, g, t < n ? a.Dk : 0, a.vec_k, x);
-    kt[kb] = split<NI>(x);
-    load8(qrow, 32 * kb, g, t < n ? a.Dk : 0, a.vec_q, x);
-    qt[kb] = split<NI>(x);
+    const int d = 32 * kb + 4 * g, left = t < n ? a.Dk - d : 0;
+    kt[kb] = split<NI>(fetched<T>(kr[kb][0], left), fetched<T>(kr[kb][1], left - 16));
     store_terms<NI>(kq[0] + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
-    store_terms<NI>(kq[1] + (w * KB + kb) * NI * kFrag, lane, qt[kb]);
+    if constexpr (BWD)
+      store_terms<NI>(kq[1] + (w * KB + kb) * NI * kFrag, lane,
+                      split<NI>(fetched<T>(qr[kb][0], left), fetched<T>(qr[kb][1], left - 16)));
   }
   __syncthreads();
-  if (h % a.group == 0) {
-    __bf16* out = key_tiles<KB, NI>(a, tile, hk);
-    constexpr int kAll = 4 * KB * NI * kFrag;
+  if constexpr (BWD) {
+    if (h % a.group == 0) {
+      __bf16* out = key_tiles<KB, NI>(a, tile, hk);
+      constexpr int kAll = 4 * KB * NI * kFrag;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      store_terms<NI>(out + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
-      if (!BWD) store_terms<NI>(out + 2 * kAll + (w * KB + kb) * NI * kFrag, lane, qt[kb]);
-    }
-    // Transposed: rows are channels, inner indices tokens.
-    for (int f = w; f < 4 * KB; f += 4) {
-      const int d = 16 * (f / 2) + m, tb = 32 * (f & 1);
-      const int src = (d / 32) * NI * kFrag + (d & 3) + ((d >> 4) & 1) * 4;
-      const int sl = 16 * ((d >> 2) & 3);
+      for (int kb = 0; kb < KB; ++kb) store_terms<NI>(out + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
+      for (int f = w; f < 4 * KB; f += 4)
 #pragma unroll
-      for (int x = 0; x < (BWD ? 2 : 1); ++x) {
-        Terms<NI> r;
-#pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int tok = tb + 4 * g + (i & 3) + 16 * (i >> 2);
-            r.t[j][i] = kq[x][(tok >> 4) * KB * NI * kFrag + src + j * kFrag + (sl + (tok & 15)) * 8];
-          }
-        store_terms<NI>(out + (1 + x) * kAll + f * NI * kFrag, lane, r);
-      }
+        for (int x = 0; x < 2; ++x)
+          store_terms<NI>(out + (1 + x) * kAll + f * NI * kFrag, lane, transposed<KB, NI>(kq[x], f, lane));
     }
   }
   // A for tokens i of this wavefront, lane m = column j (read by rows below).
-  __bf16* tri = tri_tiles<T>(a, tile, h);
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (jt <= w) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) acc = product<2>(kt[kb], load_terms<NI>(kq[0] + (jt * KB + kb) * NI * kFrag, lane), acc);
+      settle(acc);
     }
     const int j = 16 * jt + m;
 #pragma unroll
@@ -217,29 +231,28 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       As[i * LD + j] = j < i ? bs[i] * fade(Gs[i] - Gs[j]) * acc[x] : 0.f;
     }
   }
-  // P: rows i of this wavefront (BWD: transposed, rows j of this wavefront).
+  if constexpr (BWD) {  // P transposed: rows j of this wavefront
+    __bf16* tri = tri_tiles(a, tile, h);
 #pragma unroll
-  for (int kb2 = 0; kb2 < 2; ++kb2) {
-    if (BWD ? kb2 < w / 2 : kb2 > w / 2) continue;
-    f32x4 p[2];
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+      if (kb2 < w / 2) continue;
+      f32x4 p[2];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int ot = 2 * kb2 + x;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < 2; ++x) {
+        const int it = 2 * kb2 + x;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const Terms<NI> y = load_terms<NI>(kq[BWD ? 1 : 0] + (ot * KB + kb) * NI * kFrag, lane);
-        acc = product<2>(y, BWD ? kt[kb] : qt[kb], acc);
+        for (int kb = 0; kb < KB; ++kb)
+          acc = product<2>(load_terms<NI>(kq[1] + (it * KB + kb) * NI * kFrag, lane), kt[kb], acc);
+        settle(acc);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = 16 * w + m, i = 16 * it + 4 * g + r;
+          p[x][r] = j <= i ? a.scale * fade(Gs[i] - Gs[j]) * acc[r] : 0.f;
+        }
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int mine = 16 * w + m, other = 16 * ot + 4 * g + r;
-        const int i = BWD ? other : mine, j = BWD ? mine : other;
-        p[x][r] = j <= i ? a.scale * fade(Gs[i] - Gs[j]) * acc[r] : 0.f;
-      }
+      store_terms<NX>(tri + (kTri + tri_upper(w, kb2)) * NX * kFrag, lane, split<NX>(p[0], p[1]));
     }
-    const int f = BWD ? tri_upper(w, kb2) : tri_lower(w, kb2);
-    store_terms<NO>(tri + (kTri * NX + f * NO) * kFrag, lane, split<NO>(p[0], p[1]));
   }
   __syncthreads();
   // T = (I + A)^-1.  The 16 x 16 diagonal blocks by forward substitution, a column per
@@ -280,6 +293,7 @@ __global__ __launch_bounds__(256) void prep(Args a) {
         const float* r = Ts + (16 * it + m) * LD + 16 * it + 4 * g;
 #pragma unroll
         for (int x = 0; x < 4; ++x) z = __builtin_amdgcn_mfma_f32_16x16x4f32(r[x], -y[x], z, 0, 0, 0);
+        settle(z);
         col[d] = z;
 #pragma unroll
         for (int x = 0; x < 4; ++x) Ts[(16 * it + 4 * g + x) * LD + 16 * w + m] = z[x];
@@ -290,14 +304,19 @@ __global__ __launch_bounds__(256) void prep(Args a) {
 #pragma unroll
   for (int kb2 = 0; kb2 < 2; ++kb2) {
     if (BWD ? kb2 < w / 2 : kb2 > w / 2) continue;
-    float x[8];
+    f32x4 x[2];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int o = 32 * kb2 + 4 * g + (i & 3) + 16 * (i >> 2);
-      x[i] = BWD ? Ts[o * LD + t] : Ts[t * LD + o];
+      x[i >> 2][i & 3] = BWD ? Ts[o * LD + t] : Ts[t * LD + o];
     }
-    const int f = BWD ? tri_upper(w, kb2) : tri_lower(w, kb2);
-    store_terms<NX>(tri + f * NX * kFrag, lane, split<NX>(x));
+    if constexpr (BWD) {
+      store_terms<NX>(tri_tiles(a, tile, h) + tri_upper(w, kb2) * NX * kFrag, lane, split<NX>(x[0], x[1]));
+    } else {
+      float* out = a.inv + ((tile * a.H + h) * kTri + tri_lower(w, kb2)) * (int64_t)kFrag + lane * 4;
+      *reinterpret_cast<f32x4*>(out) = x[0];
+      *reinterpret_cast<f32x4*>(out + 256) = x[1];
+    }
   }
 }
 
@@ -307,7 +326,7 @@ __global__ __launch_bounds__(256) void prep(Args a) {
 // A chunk token by token, for the chunks that hold a value that is not finite: a
 // product with the zeros of T and P would carry it to earlier tokens.
 template <typename T, int KB, bool SAVE>
-__device__ __noinline__ void chunk_by_token(const Args& a, const Rows& rows, int64_t row0, int n, int h, int col,
+__device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, int64_t row0, int n, int h, int col,
                                             int64_t tile, f32x4 (&S)[2 * KB]) {
   const int hk = h / a.group, lane = threadIdx.x & 63, g = lane >> 4;
   for (int t = 0; t < n; ++t) {
@@ -318,7 +337,7 @@ __device__ __noinline__ void chunk_by_token(const Args& a, const Rows& rows, int
     float x = 0.f;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      const f32x4 k = load4(krow + 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g, a.vec_k);
+      const f32x4 k = load4(krow, 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (16 * dt + 4 * g + i < a.Dk) {
@@ -333,8 +352,8 @@ __device__ __noinline__ void chunk_by_token(const Args& a, const Rows& rows, int
     float o = 0.f;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      const f32x4 k = load4(krow + 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g, a.vec_k);
-      const f32x4 q = load4(qrow + 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g, a.vec_q);
+      const f32x4 k = load4(krow, 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g);
+      const f32x4 q = load4(qrow, 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (16 * dt + 4 * g + i < a.Dk) {
@@ -346,143 +365,270 @@ __device__ __noinline__ void chunk_by_token(const Args& a, const Rows& rows, int
     o = group_sum(o);
     if (g == 0 && col < a.Dv) {
       ((T*)a.o)[rows.batch * a.ob + h * a.oh + (row0 + t) * a.on + col] = (T)(a.scale * o);
-      if (SAVE) a.us[((tile * a.H + h) * C + t) * a.Dv + col] = u;
+      if (SAVE) a.us[(((tile * a.H + h) * a.groups + col / 16) * 4 + t / 16) * 256 + (16 * ((t & 15) / 4) + (col & 15)) * 4 + (t & 3)] = u;
     }
   }
 }
 
-template <typename T, int KB, bool SAVE>
-__global__ __launch_bounds__(256) void chain(Args a) {
+// A workgroup has 16 NW columns of one head's state: NW wavefronts that keep 16 each
+// (in registers, 32 bits), and four that feed them and write o.  What one chunk
+// costs is the chain S -> K S -> R -> U -> S, so everything else is taken off it:
+// the feeders fetch the next chunk's rows, lay K and its transpose out as operand
+// tiles in LDS, split T, and compute P and o (from S and U, which the chain leaves in
+// LDS as terms).  Two barriers per chunk, so that one buffer each is enough:
+//   first part   chain: splits S, K S          feeders: T, V and K' of this chunk to LDS,
+//                                              P of this chunk, o of the one before
+//   second part  chain: R, U, S                feeders: q S of this chunk, K of the next to LDS
+template <typename T, int KB, int NW, bool SAVE>
+__global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>, ORD = kOutOrder<T>;
+  __shared__ __bf16 Kf[4 * KB * NI * kFrag], Kt[4 * KB * NI * kFrag], Tf[kTri * NX * kFrag];
+  __shared__ T Vf[NW * 4 * 256];
+  __shared__ __bf16 Sf[NW * KB * NO * kFrag], Uf[NW * 2 * NO * kFrag];
+  __shared__ float vecs[2][V_COUNT * C];
+  __shared__ int by_token[NW];
   const int64_t seq = blockIdx.x;
   const int h = blockIdx.y, hk = h / a.group;
-  const int wave = blockIdx.z * (blockDim.x / 64) + threadIdx.x / 64;
-  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  if (16 * wave >= a.Dv) return;
-  const int col = 16 * wave + m;
-  const bool in = col < a.Dv;
+  const int wave = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const Rows rows = rows_of(a.cu, seq, a.N);
   const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), nch = (rows.n + C - 1) / C;
-  f32x4 S[2 * KB];
-#pragma unroll
-  for (int dt = 0; dt < 2 * KB; ++dt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 16 * dt + 4 * g + i;
-      S[dt][i] = a.init && in && d < a.Dk ? a.init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
-    }
-  for (int64_t c = 0; c < nch; ++c) {
-    const int64_t tile = tile0 + c, row0 = rows.first + c * C;
-    const int n = rows.n - c * C < C ? (int)(rows.n - c * C) : C;
-    if (SAVE) {
-#pragma unroll
-      for (int dt = 0; dt < 2 * KB; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = 16 * dt + 4 * g + i;
-          if (in && d < a.Dk) a.states[((tile * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
-        }
-    }
-    constexpr int kAll = 4 * KB * NI * kFrag;
-    const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
-    const __bf16* tri = tri_tiles<T>(a, tile, h);
-    const float* vec = vec_of(a, tile, h);
-    Terms<NX> s[KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
-    // R
-    f32x4 R[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) x = product<2>(load_terms<NI>(kf + (mt * KB + kb) * NI * kFrag, lane), s[kb], x);
-      const f32x4 bg = *reinterpret_cast<const f32x4*>(vec + V_BG * C + 16 * mt + 4 * g);
-      const f32x4 b = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * mt + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * mt + 4 * g + i;
-        const float v =
-            t < n && in ? (float)((const T*)a.v)[rows.batch * a.vb + h * a.vh + (row0 + t) * a.vn + col] : 0.f;
-        R[mt][i] = b[i] * v - bg[i] * x[i];
-      }
-    }
-    // U
-    Terms<NX> r[2] = {split<NX>(R[0], R[1]), split<NX>(R[2], R[3])};
-    f32x4 U[4];
-    float odd = 0.f;
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb <= mt / 2; ++kb) x = product<2>(load_terms<NX>(tri + tri_lower(mt, kb) * NX * kFrag, lane), r[kb], x);
-      U[mt] = x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) odd += 0.f * x[i];
-    }
-    // o, transposed: lane m has token 16 mt + m and columns 4g..4g+3 of the wavefront's
-    const Terms<NO> u[2] = {split<NO>(U[0], U[1]), split<NO>(U[2], U[3])};
-    f32x4 O[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        Terms<NO> so;
-#pragma unroll
-        for (int j = 0; j < NO; ++j) so.t[j] = s[kb].t[j];
-        x = product<ORD>(so, load_terms<NI>(kf + 2 * kAll + (mt * KB + kb) * NI * kFrag, lane), x);
-      }
-#pragma unroll
-      for (int kb = 0; kb <= mt / 2; ++kb)
-        y = product<ORD>(u[kb], load_terms<NO>(tri + (kTri * NX + tri_lower(mt, kb) * NO) * kFrag, lane), y);
-      const float since = a.scale * vec[V_SINCE * C + 16 * mt + m];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        O[mt][i] = since * x[i] + y[i];
-        odd += 0.f * O[mt][i];
-      }
-    }
-    if (__any(odd != 0.f)) {  // NaN: something is not finite
-      chunk_by_token<T, KB, SAVE>(a, rows, row0, n, h, col, tile, S);
-      continue;
-    }
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const int t = 16 * mt + m;
-      if (t < n)
-        store4((T*)a.o + rows.batch * a.ob + h * a.oh + (row0 + t) * a.on + 16 * wave + 4 * g, O[mt],
-               a.Dv - 16 * wave - 4 * g, a.vec_o);
-    }
-    if (SAVE) {
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (in) a.us[((tile * a.H + h) * C + 16 * mt + 4 * g + i) * a.Dv + col] = U[mt][i];
-    }
-    // S
-    const float whole = vec[V_SINCE * C + C - 1];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) U[mt] *= *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
-    const Terms<NX> ul[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
-#pragma unroll
-    for (int dt = 0; dt < 2 * KB; ++dt) {
-      S[dt] *= whole;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        S[dt] = product<2>(load_terms<NI>(kf + kAll + (dt * 2 + kb) * NI * kFrag, lane), ul[kb], S[dt]);
-    }
-  }
-  if (a.final) {
+  const int col0 = blockIdx.z * 16 * NW;
+  if (wave < NW) {
+    const int col = col0 + 16 * wave + m;
+    const bool in = col < a.Dv, any = col0 + 16 * wave < a.Dv;
+    f32x4 S[2 * KB];
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 16 * dt + 4 * g + i;
-        if (in && d < a.Dk) a.final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+        S[dt][i] = a.init && in && d < a.Dk ? a.init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
       }
+    if (nch) lds_barrier();
+    for (int64_t c = 0; c < nch; ++c) {
+      const int64_t tile = tile0 + c;
+      const int64_t cg = (tile * a.H + h) * a.groups + (col0 >> 4) + wave;
+      const float* vec = vecs[c & 1];
+      f32x4 X[4];
+      if (any) {
+        if (SAVE) {
+#pragma unroll
+          for (int dt = 0; dt < 2 * KB; ++dt) *reinterpret_cast<f32x4*>(a.states + (cg * 2 * KB + dt) * 256 + lane * 4) = S[dt];
+        }
+        Terms<NX> s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+#pragma unroll
+          for (int j = 0; j < NO; ++j)
+            *reinterpret_cast<bf16x8*>(Sf + ((wave * KB + kb) * NO + j) * kFrag + lane * 8) = s[kb].t[j];
+        }
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          X[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) X[mt] = product<2>(load_terms<NI>(Kf + (mt * KB + kb) * NI * kFrag, lane), s[kb], X[mt]);
+        }
+        settle(X);
+      }
+      lds_barrier();
+      if (any) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          const f32x4 bg = *reinterpret_cast<const f32x4*>(vec + V_BG * C + 16 * mt + 4 * g);
+          const f32x4 b = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * mt + 4 * g);
+          const f32x4 v = load4(Vf, (wave * 4 + mt) * 256 + lane * 4, 4);
+          X[mt] = b * v - bg * X[mt];
+        }
+        const Terms<NX> r[2] = {split<NX>(X[0], X[1]), split<NX>(X[2], X[3])};
+        f32x4 U[4];
+        float odd = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kb = 0; kb <= mt / 2; ++kb) x = product<2>(load_terms<NX>(Tf + tri_lower(mt, kb) * NX * kFrag, lane), r[kb], x);
+          U[mt] = x;
+        }
+        settle(U);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) odd += 0.f * U[mt][i];
+        const bool slow = __any(odd != 0.f);  // NaN: something is not finite
+        if (lane == 0) by_token[wave] = slow;
+        if (slow) {
+          chunk_by_token<T, KB, SAVE>(a, rows, rows.first + c * C, rows.n - c * C < C ? (int)(rows.n - c * C) : C, h, col,
+                                      tile, S);
+        } else {
+          if (SAVE) {
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) *reinterpret_cast<f32x4*>(a.us + (cg * 4 + mt) * 256 + lane * 4) = U[mt];
+          }
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const Terms<NO> u = split<NO>(U[2 * kb], U[2 * kb + 1]);
+            store_terms<NO>(Uf + (wave * 2 + kb) * NO * kFrag, lane, u);
+          }
+          const float whole = vec[V_SINCE * C + C - 1];
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) U[mt] *= *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
+          const Terms<NX> ul[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
+#pragma unroll
+          for (int dt = 0; dt < 2 * KB; ++dt) {
+            S[dt] *= whole;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) S[dt] = product<2>(load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane), ul[kb], S[dt]);
+          }
+          settle(S);
+        }
+      }
+      lds_barrier();
+    }
+    if (a.final) {
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 16 * dt + 4 * g + i;
+          if (in && d < a.Dk) a.final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+        }
+    }
+    return;
   }
+  if (!nch) return;
+  // A feeder: tokens 16w + m of each chunk.
+  const int w = wave - NW, t = 16 * w + m, ft = threadIdx.x - 64 * NW;
+  const T* kbase = (const T*)a.k + rows.batch * a.kb + hk * a.kh + rows.first * a.kn;
+  const T* qbase = (const T*)a.q + rows.batch * a.qb + hk * a.qh + rows.first * a.qn;
+  const T* vbase = (const T*)a.v + rows.batch * a.vb + h * a.vh + rows.first * a.vn;
+  T* obase = (T*)a.o + rows.batch * a.ob + h * a.oh + rows.first * a.on;
+  // V: four lanes per token, 4 NW columns each; T: three tile halves per wavefront.
+  const int vt = 16 * w + (lane >> 2), vc = (lane & 3) * 4 * NW;
+  Raw4<T> kr[KB][2], qr[KB][2], vr[NW];
+  f32x4 tr[3], er;
+  const auto fetch = [&](int64_t c) {
+    const int64_t row = c * C + t;
+    const int dk = row < rows.n ? a.Dk : 0;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int d = 32 * kb + 16 * x + 4 * g;
+        kr[kb][x] = fetch4(kbase, row * a.kn + d, dk - d);
+        qr[kb][x] = fetch4(qbase, row * a.qn + d, dk - d);
+      }
+    const int64_t vrow = c * C + vt;
+    const int dv = vrow < rows.n ? a.Dv - col0 - vc : 0;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) vr[x] = fetch4(vbase, vrow * a.vn + col0 + vc + 4 * x, dv - 4 * x);
+    const float* inv = a.inv + ((tile0 + c) * a.H + h) * (int64_t)(kTri * kFrag);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) tr[x] = *reinterpret_cast<const f32x4*>(inv + (3 * w + x) * 256 + lane * 4);
+    er = *reinterpret_cast<const f32x4*>(vec_of(a, tile0 + c, h) + (ft % (V_COUNT * C / 4)) * 4);
+  };
+  // What the lane fetched of a row of K or Q of chunk c.
+  const auto row_terms = [&](const Raw4<T> (&x)[2], int kb, int64_t c) {
+    const int left = c * C + t < rows.n ? a.Dk - 32 * kb - 4 * g : 0;
+    return split<NI>(fetched<T>(x[0], left), fetched<T>(x[1], left - 16));
+  };
+  const auto put_keys = [&](int64_t c) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) store_terms<NI>(Kf + (w * KB + kb) * NI * kFrag, lane, row_terms(kr[kb], kb, c));
+    if (ft < V_COUNT * C / 4) *reinterpret_cast<f32x4*>(vecs[c & 1] + ft * 4) = er;
+  };
+  fetch(0);
+  put_keys(0);
+  lds_barrier();
+  Terms<NO> p[2];  // P of the last chunk: lane m = token i, inner indices j
+  f32x4 O[NW];     // scale e^G S' q of it
+  const auto write_out = [&](int64_t c) {
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      if (col0 + 16 * x >= a.Dv) continue;
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        if (kb <= w / 2) {
+          y = product<ORD>(load_terms<NO>(Uf + (x * 2 + kb) * NO * kFrag, lane), p[kb], y);
+          settle(y);
+        }
+      if (c * C + t < rows.n && !by_token[x] && col0 + 16 * x + 4 * g < a.Dv)
+        store4(obase + (c * C + t) * a.on + col0 + 16 * x + 4 * g, O[x] + y);
+    }
+  };
+  for (int64_t c = 0; c < nch; ++c) {
+    const float* vec = vecs[c & 1];
+    // T and V
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      const int f = 3 * w + x;
+      f32x4 y = tr[x];
+#pragma unroll
+      for (int j = 0; j < NX; ++j) {
+        bf16x4 e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = j + 1 < NX ? (__bf16)upper_half(y[i]) : (__bf16)y[i];
+          if (j + 1 < NX) y[i] -= upper_half(y[i]);
+        }
+        *reinterpret_cast<bf16x4*>(Tf + ((f >> 1) * NX + j) * kFrag + lane * 8 + 4 * (f & 1)) = e;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < NW; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int cc = vc + 4 * x + i;
+        Vf[((cc >> 4) * 4 + w) * 256 + (16 * ((vt & 15) >> 2) + (cc & 15)) * 4 + (vt & 3)] =
+            c * C + vt < rows.n && col0 + cc < a.Dv ? vr[x][i] : (T)0.f;
+      }
+    for (int f = w; f < 4 * KB; f += 4) store_terms<NI>(Kt + f * NI * kFrag, lane, transposed<KB, NI>(Kf, f, lane));
+    Terms<NI> q[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) q[kb] = row_terms(qr[kb], kb, c);
+    if (c + 1 < nch) fetch(c + 1);
+    if (c) write_out(c - 1);
+    // P
+    const float Gt = vec[V_G * C + t], Gl = vec[V_GLOW * C + t];
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+      if (kb2 > w / 2) continue;
+      f32x4 y[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int jt = 2 * kb2 + x;
+        y[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (jt <= w) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) y[x] = product<2>(load_terms<NI>(Kf + (jt * KB + kb) * NI * kFrag, lane), q[kb], y[x]);
+          settle(y[x]);
+          const f32x4 G = *reinterpret_cast<const f32x4*>(vec + V_G * C + 16 * jt + 4 * g);
+          const f32x4 L = *reinterpret_cast<const f32x4*>(vec + V_GLOW * C + 16 * jt + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * jt + 4 * g + r;
+            y[x][r] = j <= t ? a.scale * expf((Gt - G[r]) + (Gl - L[r])) * y[x][r] : 0.f;
+          }
+        }
+      }
+      p[kb2] = split<NO>(y[0], y[1]);
+    }
+    lds_barrier();
+    const float since = a.scale * vec[V_SINCE * C + t];
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      O[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (col0 + 16 * x >= a.Dv) continue;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) O[x] = product<ORD>(load_terms<NO>(Sf + (x * KB + kb) * NO * kFrag, lane), q[kb], O[x]);
+      settle(O[x]);
+      O[x] *= since;
+    }
+    if (c + 1 < nch) put_keys(c + 1);
+    lds_barrier();
+  }
+  write_out(nch - 1);
 }
 
 // --------------------------------------------------------------------------
@@ -502,10 +648,10 @@ __global__ __launch_bounds__(256) void chain(Args a) {
 // --------------------------------------------------------------------------
 template <typename T, int KB>
 __global__ __launch_bounds__(256) void chain_back(Args a) {
-  constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>;
+  constexpr int NI = kInputTerms<T>;
   const int64_t seq = blockIdx.x;
   const int h = blockIdx.y, hk = h / a.group;
-  const int wave = blockIdx.z * (blockDim.x / 64) + threadIdx.x / 64;
+  const int wave = blockIdx.z * (blockDim.x / 64) + wave_index();
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   if (16 * wave >= a.Dv) return;
   const int col = 16 * wave + m;
@@ -523,16 +669,12 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
   for (int64_t c = nch - 1; c >= 0; --c) {
     const int64_t tile = tile0 + c, row0 = rows.first + c * C;
     const int n = rows.n - c * C < C ? (int)(rows.n - c * C) : C;
+    const int64_t cg = (tile * a.H + h) * a.groups + wave;
 #pragma unroll
-    for (int dt = 0; dt < 2 * KB; ++dt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = 16 * dt + 4 * g + i;
-        if (in && d < a.Dk) a.dstates[((tile * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
-      }
+    for (int dt = 0; dt < 2 * KB; ++dt) *reinterpret_cast<f32x4*>(a.dstates + (cg * 2 * KB + dt) * 256 + lane * 4) = S[dt];
     constexpr int kAll = 4 * KB * NI * kFrag;
     const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
-    const __bf16* tri = tri_tiles<T>(a, tile, h);
+    const __bf16* tri = tri_tiles(a, tile, h);
     const float* vec = vec_of(a, tile, h);
     f32x4 dO[4];
 #pragma unroll
@@ -553,12 +695,14 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) x = product<2>(load_terms<NI>(kf + (mt * KB + kb) * NI * kFrag, lane), s[kb], x);
+      settle(x);
       x *= *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
 #pragma unroll
       for (int kb = mt / 2; kb < 2; ++kb)
-        x = product<2>(load_terms<NO>(tri + (kTri * NX + tri_upper(mt, kb) * NO) * kFrag, lane), o[kb], x);
+        x = product<2>(load_terms<NX>(tri + (kTri + tri_upper(mt, kb)) * NX * kFrag, lane), o[kb], x);
       U[mt] = x;
     }
+    settle(U);
     const Terms<NX> u[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
     f32x4 R[4];
 #pragma unroll
@@ -566,13 +710,14 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kb = mt / 2; kb < 2; ++kb) x = product<2>(load_terms<NX>(tri + tri_upper(mt, kb) * NX * kFrag, lane), u[kb], x);
+      settle(x);
       R[mt] = x;
+      *reinterpret_cast<f32x4*>(a.drs + (cg * 4 + mt) * 256 + lane * 4) = x;
       const f32x4 b = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * mt + 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int t = 16 * mt + 4 * g + i;
         if (in) {
-          a.drs[((tile * a.H + h) * C + t) * a.Dv + col] = x[i];
           if (t < n) ((T*)a.dv)[rows.batch * a.dvb + h * a.dvh + (row0 + t) * a.dvn + col] = (T)(b[i] * x[i]);
         }
       }
@@ -595,6 +740,7 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
         S[dt] = product<2>(load_terms<NI>(kf + 2 * kAll + (dt * 2 + kb) * NI * kFrag, lane), e[kb], S[dt]);
       }
     }
+    settle(S);
   }
   if (a.d_init) {
 #pragma unroll
@@ -607,6 +753,26 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
   }
 }
 
+// One lane's eight values of a row: inner indices k0 + 4g + i and k0 + 16 + 4g + i, zero from
+// index `width` on.
+template <typename T>
+__device__ __forceinline__ void load8(const T* base, int64_t at, int k0, int g, int width, float (&x)[8]) {
+  const int d = k0 + 4 * g;
+  const f32x4 lo = load4(base, at + d, width - d), hi = load4(base, at + d + 16, width - d - 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
+}
+
+// Row r, columns c0 + 4g.. and c0 + 16 + 4g.. of a matrix that chain() or chain_back() kept as it
+// lay in registers, `tiles` tiles of 16 rows for each of the 16-column groups.
+__device__ __forceinline__ void load_kept(const float* x, int tiles, int r, int c0, int g, int groups, float (&y)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int cg = c0 / 16 + (i >> 2);
+    y[i] = cg < groups ? x[(cg * tiles + r / 16) * 256 + (16 * ((r & 15) / 4) + 4 * g + (i & 3)) * 4 + (r & 3)] : 0.f;
+  }
+}
+
 // Grid (tiles, Hk), four wavefronts; wavefront w has tokens 16w..16w+15, lane m the token
 // 16w + m, and channels 4g.. of each 16-channel tile: no product crosses wavefronts.
 template <typename T, int KB>
@@ -616,7 +782,7 @@ __global__ __launch_bounds__(256) void grads(Args a) {
   __shared__ float dGs[C], ends[4];
   const int64_t tile = blockIdx.x;
   const int hk = blockIdx.y;
-  const int w = threadIdx.x / 64, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int w = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   zero_outside<C>(a.cu, a.sequences, tile, a.N, (T*)a.dq + hk * a.dqh, a.dqn, a.Dk, threadIdx.x, 256);
   zero_outside<C>(a.cu, a.sequences, tile, a.N, (T*)a.dk + hk * a.dkh, a.dkn, a.Dk, threadIdx.x, 256);
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
@@ -635,11 +801,9 @@ __global__ __launch_bounds__(256) void grads(Args a) {
   for (int dt = 0; dt < 2 * KB; ++dt) dq[dt] = dk[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
     const float* vec = vec_of(a, tile, h);
-    const float* St = a.states + (tile * a.H + h) * (int64_t)a.Dk * a.Dv;
-    const float* dSt = a.dstates + (tile * a.H + h) * (int64_t)a.Dk * a.Dv;
-    const float* Us = a.us + (tile * a.H + h) * (int64_t)C * a.Dv;
-    const float* Rs = a.drs + (tile * a.H + h) * (int64_t)C * a.Dv;
-    const bool vec_f = a.Dv % 4 == 0;
+    const int64_t cg = (tile * a.H + h) * a.groups;
+    const float *St = a.states + cg * 2 * KB * 256, *dSt = a.dstates + cg * 2 * KB * 256;
+    const float *Us = a.us + cg * 4 * 256, *Rs = a.drs + cg * 4 * 256;
     f32x4 hq[2 * KB], rho[2 * KB], kw[2 * KB];
     f32x4 E1[4], E2[4], F1[4], F2[4];  // dO_i.u_j and dR_i.u_j: lane = i, rows j <= i; lane = j, rows i >= j
 #pragma unroll
@@ -649,10 +813,10 @@ __global__ __launch_bounds__(256) void grads(Args a) {
     float db = 0.f, ss = 0.f;
     for (int c0 = 0; c0 < a.Dv; c0 += 32) {
       float xo[8], xr[8], xu[8], xv[8];
-      load8((const T*)a.d_o + bt * a.dob + h * a.doh + (row0 + t) * a.don, c0, g, t < n ? a.Dv : 0, a.vec_do, xo);
-      load8((const T*)a.v + bt * a.vb + h * a.vh + (row0 + t) * a.vn, c0, g, t < n ? a.Dv : 0, a.vec_v, xv);
-      load8(Rs + t * (int64_t)a.Dv, c0, g, t < n ? a.Dv : 0, vec_f, xr);
-      load8(Us + t * (int64_t)a.Dv, c0, g, t < n ? a.Dv : 0, vec_f, xu);
+      load8((const T*)a.d_o + bt * a.dob + h * a.doh + row0 * a.don, t * a.don, c0, g, t < n ? a.Dv : 0, xo);
+      load8((const T*)a.v + bt * a.vb + h * a.vh + row0 * a.vn, t * a.vn, c0, g, t < n ? a.Dv : 0, xv);
+      load_kept(Rs, 4, t, c0, g, t < n ? a.groups : 0, xr);
+      load_kept(Us, 4, t, c0, g, t < n ? a.groups : 0, xu);
 #pragma unroll
       for (int i = 0; i < 8; ++i) db = fmaf(xr[i], xv[i], db);
       const Terms<NI> o = split<NI>(xo);
@@ -661,8 +825,8 @@ __global__ __launch_bounds__(256) void grads(Args a) {
       for (int dt = 0; dt < 2 * KB; ++dt) {
         const int d = 16 * dt + m;
         float xs[8], xd[8];
-        load8(St + d * (int64_t)a.Dv, c0, g, d < a.Dk ? a.Dv : 0, vec_f, xs);
-        load8(dSt + d * (int64_t)a.Dv, c0, g, d < a.Dk ? a.Dv : 0, vec_f, xd);
+        load_kept(St, 2 * KB, d, c0, g, a.groups, xs);
+        load_kept(dSt, 2 * KB, d, c0, g, a.groups, xd);
         if (dt % 4 == w) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) ss = fmaf(xs[i], xd[i], ss);
@@ -672,22 +836,25 @@ __global__ __launch_bounds__(256) void grads(Args a) {
         rho[dt] = product<2>(s, r, rho[dt]);
         kw[dt] = product<2>(ds, u, kw[dt]);
       }
+      settle(hq), settle(rho), settle(kw);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int y = 16 * x + m;
         if (x <= w) {
           float z[8];
-          load8(Us + y * (int64_t)a.Dv, c0, g, y < n ? a.Dv : 0, vec_f, z);
+          load_kept(Us, 4, y, c0, g, y < n ? a.groups : 0, z);
           const Terms<NX> uj = split<NX>(z);
           E1[x] = product<2>(uj, o, E1[x]);
           E2[x] = product<2>(uj, r, E2[x]);
+          settle(E1[x]), settle(E2[x]);
         }
         if (x >= w) {
           float z[8];
-          load8((const T*)a.d_o + bt * a.dob + h * a.doh + (row0 + y) * a.don, c0, g, y < n ? a.Dv : 0, a.vec_do, z);
+          load8((const T*)a.d_o + bt * a.dob + h * a.doh + row0 * a.don, y * a.don, c0, g, y < n ? a.Dv : 0, z);
           F1[x] = product<2>(split<NI>(z), u, F1[x]);
-          load8(Rs + y * (int64_t)a.Dv, c0, g, y < n ? a.Dv : 0, vec_f, z);
+          load_kept(Rs, 4, y, c0, g, y < n ? a.groups : 0, z);
           F2[x] = product<2>(split<NX>(z), u, F2[x]);
+          settle(F1[x]), settle(F2[x]);
         }
       }
     }
@@ -695,14 +862,14 @@ __global__ __launch_bounds__(256) void grads(Args a) {
     const float since = vec[V_SINCE * C + t], left = vec[V_LEFT * C + t], whole = vec[V_SINCE * C + C - 1];
     // k.(the state's part of kw), q.dq, k.rho, k.kw
     float kend = 0.f, qq = 0.f, kr = 0.f, kk = 0.f;
-    const T* krow = (const T*)a.k + bt * a.kb + hk * a.kh + (row0 + t) * a.kn;
-    const T* qrow = (const T*)a.q + bt * a.qb + hk * a.qh + (row0 + t) * a.qn;
+    const T* kbase = (const T*)a.k + bt * a.kb + hk * a.kh + row0 * a.kn;
+    const T* qbase = (const T*)a.q + bt * a.qb + hk * a.qh + row0 * a.qn;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
       hq[dt] *= a.scale * since;
       rho[dt] *= -since;
       kw[dt] *= left;
-      const f32x4 k = load4(krow + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0, a.vec_k);
+      const f32x4 k = load4(kbase, t * a.kn + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) kend = fmaf(k[i], kw[dt][i], kend);
     }
@@ -733,18 +900,20 @@ __global__ __launch_bounds__(256) void grads(Args a) {
         if (lo) {
           hq[dt] = product<2>(kT, e1, hq[dt]);
           rho[dt] = product<2>(kT, e2, rho[dt]);
+          settle(hq[dt]), settle(rho[dt]);
         }
         if (hi) {
           const Terms<NI> qT = load_terms<NI>(kf + 2 * kAll + (dt * 2 + kb) * NI * kFrag, lane);
           kw[dt] = product<2>(qT, f1, kw[dt]);
           kw[dt] = product<2>(kT, f2, kw[dt]);
+          settle(kw[dt]);
         }
       }
     }
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      const f32x4 k = load4(krow + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0, a.vec_k);
-      const f32x4 q = load4(qrow + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0, a.vec_q);
+      const f32x4 k = load4(kbase, t * a.kn + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0);
+      const f32x4 q = load4(qbase, t * a.qn + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         qq = fmaf(q[i], hq[dt][i], qq);
@@ -784,8 +953,9 @@ __global__ __launch_bounds__(256) void grads(Args a) {
     T* dkrow = (T*)a.dk + bt * a.dkb + hk * a.dkh + (row0 + t) * a.dkn;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      store4(dqrow + 16 * dt + 4 * g, dq[dt], a.Dk - 16 * dt - 4 * g, a.vec_dq);
-      store4(dkrow + 16 * dt + 4 * g, dk[dt], a.Dk - 16 * dt - 4 * g, a.vec_dk);
+      if (16 * dt + 4 * g >= a.Dk) continue;
+      store4(dqrow + 16 * dt + 4 * g, dq[dt]);
+      store4(dkrow + 16 * dt + 4 * g, dk[dt]);
     }
   }
 }
@@ -796,6 +966,27 @@ __global__ __launch_bounds__(256) void grads(Args a) {
 //     x = k'S, y = q'S;  u = b (v - a x);  S <- a S + k u';  o = scale (a y + (q.k) u)
 // --------------------------------------------------------------------------
 constexpr int kStepCols = 32;
+
+// Up to four elements, n of them there.  vec: in one access where all are.
+template <typename T>
+__device__ __forceinline__ f32x4 load_some(const T* p, int n, bool vec) {
+  if (vec) return load4(p, 0, n);
+  f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) r[i] = (float)p[i];
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, f32x4 x, int n, bool vec) {
+  if (vec) {
+    if (n > 0) store4(p, x);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) p[i] = (T)x[i];
+}
 
 template <typename T, typename TO>
 __global__ __launch_bounds__(256) void step(const T* q, const T* k, const T* v, const float* gs, const float* betas,
@@ -817,7 +1008,7 @@ __global__ __launch_bounds__(256) void step(const T* q, const T* k, const T* v, 
   for (int j = 0; j < R; ++j) {
     const int r = r0 + 32 * j;
     const bool on = r < Dk;
-    S[j] = load4(in + (bh * Dk + (on ? r : 0)) * (int64_t)Dv + c, on ? Dv - c : 0, vec_in);
+    S[j] = load_some(in + (bh * Dk + (on ? r : 0)) * (int64_t)Dv + c, on ? Dv - c : 0, vec_in);
     kk[j] = on ? (float)kp[r] : 0.f;
     const float qq = on ? (float)qp[r] : 0.f;
     qk = fmaf(kk[j], qq, qk);
@@ -850,7 +1041,7 @@ __global__ __launch_bounds__(256) void step(const T* q, const T* k, const T* v, 
   }
   __syncthreads();
   qk = (dots[0] + dots[1]) + (dots[2] + dots[3]);
-  const f32x4 vv = load4(v + bh * Dv + c, Dv - c, false);
+  const f32x4 vv = load_some(v + bh * Dv + c, Dv - c, false);
   f32x4 u, o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -866,9 +1057,10 @@ __global__ __launch_bounds__(256) void step(const T* q, const T* k, const T* v, 
     if (r >= Dk) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) S[j][i] = fmaf(kk[j], u[i], S[j][i]);
-    store4(out_state + (bh * Dk + r) * (int64_t)Dv + c, S[j], Dv - c, vec_out);
+    store_some(out_state + (bh * Dk + r) * (int64_t)Dv + c, S[j], Dv - c, vec_out);
   }
-  if (threadIdx.x < 8) store4(out + bh * Dv + c, o, Dv - c, false);
+  asm volatile("" : "+v"(o));  // a multiply that rounds to 16 bits by itself would skip the rounding to 32
+  if (threadIdx.x < 8) store_some(out + bh * Dv + c, o, Dv - c, false);
 }
 
 // --------------------------------------------------------------------------
@@ -882,24 +1074,20 @@ int64_t tiles_of(const kdelta_problem* p) {
 
 int input_terms(int dtype) { return dtype == KDECAY_BF16 ? 1 : dtype == KDECAY_F16 ? 2 : 3; }
 
-struct Sizes {
-  size_t keys, tris, vecs, dstates, drs;
+struct Sizes {  // bytes
+  size_t inv, keys, tris, vecs, dstates, drs;
 };
 
 Sizes sizes_of(const kdelta_problem* p) {
-  const size_t tiles = tiles_of(p), KB = (p->Dk + 31) / 32, NI = input_terms(p->dtype);
-  const size_t NO = p->dtype == KDECAY_F32 ? 3 : 2;
+  const size_t tiles = tiles_of(p), KB = (p->Dk + 31) / 32, NI = input_terms(p->dtype), groups = (p->Dv + 15) / 16;
   Sizes s;
+  s.inv = up256(tiles * p->H * kTri * kFrag * 4);
   s.keys = up256(tiles * p->Hk * 3 * 4 * KB * NI * kFrag * 2);
-  s.tris = up256(tiles * p->H * kTri * (NX + NO) * kFrag * 2);
+  s.tris = up256(tiles * p->H * kTri * 2 * NX * kFrag * 2);
   s.vecs = up256(tiles * p->H * V_COUNT * C * 4);
-  s.dstates = up256(tiles * p->H * p->Dk * p->Dv * 4);
-  s.drs = up256(tiles * p->H * C * p->Dv * 4);
+  s.dstates = up256(tiles * p->H * groups * 2 * KB * 256 * 4);
+  s.drs = up256(tiles * p->H * groups * 4 * 256 * 4);
   return s;
-}
-
-bool aligned4(const void* p, const int64_t* st, int dtype) {
-  return ((uintptr_t)p & (dtype == KDECAY_F32 ? 15u : 7u)) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
 }
 
 int check(const kdelta_problem* p) {
@@ -918,12 +1106,15 @@ int check(const kdelta_problem* p) {
   if (!p->cu_seqlens && p->sequences != p->B) return fail(KDECAY_EINVAL, "sequences must be B without cu_seqlens");
   if (p->sequences > 0x7fffffff || tiles_of(p) > 0x7fffffff) return fail(KDECAY_ESHAPE, "too many sequences or rows");
   if (p->B && p->N && (!p->q || !p->k || !p->v || !p->g || !p->beta)) return fail(KDECAY_EINVAL, "null pointer argument");
-  if ((p->q_strides[3] != 1 && p->Dk != 1) || (p->k_strides[3] != 1 && p->Dk != 1) || (p->v_strides[3] != 1 && p->Dv != 1))
-    return fail(KDECAY_ELAYOUT, "channel (d) stride must be 1");
-  return 0;
+  if (p->Dk % 4 || p->Dv % 4)
+    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not multiples of 4", (long long)p->Dk, (long long)p->Dv);
+  if (!p->B || !p->N) return 0;
+  if (const int rc = check_rows(p->q, p->q_strides, p->dtype, "q")) return rc;
+  if (const int rc = check_rows(p->k, p->k_strides, p->dtype, "k")) return rc;
+  return check_rows(p->v, p->v_strides, p->dtype, "v");
 }
 
-Args args_of(const kdelta_problem* p, void* workspace) {
+Args args_of(const kdelta_problem* p, void* workspace, bool backward) {
   Args a = {};
   a.q = p->q, a.k = p->k, a.v = p->v, a.g = p->g, a.beta = p->beta, a.cu = p->cu_seqlens, a.init = p->init;
   a.qb = p->q_strides[0], a.qh = p->q_strides[1], a.qn = p->q_strides[2];
@@ -934,16 +1125,18 @@ Args args_of(const kdelta_problem* p, void* workspace) {
   a.N = p->N, a.sequences = p->sequences, a.tiles = tiles_of(p);
   a.Hk = (int)p->Hk, a.H = (int)p->H, a.Dk = (int)p->Dk, a.Dv = (int)p->Dv, a.group = (int)(p->H / p->Hk);
   a.scale = p->scale;
-  a.vec_q = aligned4(p->q, p->q_strides, p->dtype);
-  a.vec_k = aligned4(p->k, p->k_strides, p->dtype);
-  a.vec_v = aligned4(p->v, p->v_strides, p->dtype);
+  a.groups = (a.Dv + 15) / 16;
   const Sizes s = sizes_of(p);
   char* w = (char*)workspace;
-  a.keys = (__bf16*)w;
-  a.tris = (__bf16*)(w + s.keys);
-  a.vecs = (float*)(w + s.keys + s.tris);
-  a.dstates = (float*)(w + s.keys + s.tris + s.vecs);
-  a.drs = (float*)(w + s.keys + s.tris + s.vecs + s.dstates);
+  a.vecs = (float*)w, w += s.vecs;
+  if (!backward) {
+    a.inv = (float*)w;
+  } else {
+    a.keys = (__bf16*)w, w += s.keys;
+    a.tris = (__bf16*)w, w += s.tris;
+    a.dstates = (float*)w, w += s.dstates;
+    a.drs = (float*)w;
+  }
   return a;
 }
 
@@ -967,12 +1160,14 @@ int by_blocks(int64_t Dk, F f) {
   }
 }
 
-// Wavefronts of one workgroup of chain() and chain_back(), each with 16 columns.
-constexpr int kChainWaves = 4;
-dim3 chain_grid(const Args& a) {
-  const int waves = (a.Dv + 15) / 16;
-  return dim3((unsigned)a.sequences, a.H, (waves + kChainWaves - 1) / kChainWaves);
+// Wavefronts of one workgroup of chain_back(), each with 16 columns.
+constexpr int kBackWaves = 4;
+dim3 chain_grid(const Args& a, int waves) {
+  return dim3((unsigned)a.sequences, a.H, (a.groups + waves - 1) / waves);
 }
+// Of chain(): four, and fewer where three terms of wide keys leave no room in LDS for as many.
+template <typename T, int KB>
+constexpr int kChainWaves = sizeof(T) == 2 || KB <= 2 ? 4 : KB == 3 ? 2 : 1;
 
 }  // namespace delta
 }  // namespace kd
@@ -983,18 +1178,18 @@ using namespace kd::delta;
 extern "C" size_t kdelta_scan_workspace_bytes(const kdelta_problem* p) {
   if (check(p)) return 0;
   const Sizes s = sizes_of(p);
-  return s.keys + s.tris + s.vecs;
+  return s.vecs + s.inv;
 }
 
 extern "C" size_t kdelta_scan_bwd_workspace_bytes(const kdelta_problem* p) {
   if (check(p)) return 0;
   const Sizes s = sizes_of(p);
-  return s.keys + s.tris + s.vecs + s.dstates + s.drs;
+  return s.vecs + s.keys + s.tris + s.dstates + s.drs;
 }
 
 extern "C" size_t kdelta_scan_saved_floats(const kdelta_problem* p) {
   if (check(p)) return 0;
-  return (size_t)tiles_of(p) * p->H * (p->Dk + C) * p->Dv;
+  return (size_t)tiles_of(p) * p->H * ((p->Dv + 15) / 16) * (2 * ((p->Dk + 31) / 32) + 4) * 256;
 }
 
 extern "C" int kdelta_scan_fwd(const kdelta_problem* p, void* o, const int64_t* o_strides, float* final, float* saved,
@@ -1003,16 +1198,17 @@ extern "C" int kdelta_scan_fwd(const kdelta_problem* p, void* o, const int64_t* 
   if (p->sequences == 0) return 0;
   const bool rows = p->B && p->N;
   if (rows && (!o || !o_strides)) return fail(KDECAY_EINVAL, "null pointer argument");
-  if (rows && o_strides[3] != 1 && p->Dv != 1) return fail(KDECAY_ELAYOUT, "channel (d) stride must be 1");
+  if (rows)
+    if (const int rc = check_rows(o, o_strides, p->dtype, "o")) return rc;
   if (workspace_bytes < kdelta_scan_workspace_bytes(p) || (!workspace && rows) || ((uintptr_t)workspace & 15))
     return fail(KDECAY_EWORKSPACE, "scan workspace of %zu bytes missing, small or not 16-byte aligned",
                 kdelta_scan_workspace_bytes(p));
   if ((uintptr_t)saved & 15) return fail(KDECAY_ELAYOUT, "saved is not 16-byte aligned");
-  Args a = args_of(p, workspace);
+  Args a = args_of(p, workspace, false);
   a.o = o, a.final = final;
-  if (rows) a.ob = o_strides[0], a.oh = o_strides[1], a.on = o_strides[2], a.vec_o = aligned4(o, o_strides, p->dtype);
+  if (rows) a.ob = o_strides[0], a.oh = o_strides[1], a.on = o_strides[2];
   a.states = saved;
-  a.us = saved ? saved + (size_t)a.tiles * a.H * a.Dk * a.Dv : nullptr;
+  a.us = saved ? saved + (size_t)a.tiles * a.H * a.groups * 2 * ((a.Dk + 31) / 32) * 256 : nullptr;
   const hipStream_t s = (hipStream_t)stream;
   return by_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -1022,10 +1218,11 @@ extern "C" int kdelta_scan_fwd(const kdelta_problem* p, void* o, const int64_t* 
         prep<T, KB, false><<<dim3((unsigned)a.tiles, a.H), 256, 0, s>>>(a);
         if (const int rc = hip_check("kdelta prep launch")) return rc;
       }
+      constexpr int NW = kChainWaves<T, KB>;
       if (saved)
-        chain<T, KB, true><<<chain_grid(a), 64 * kChainWaves, 0, s>>>(a);
+        chain<T, KB, NW, true><<<chain_grid(a, NW), 64 * (NW + 4), 0, s>>>(a);
       else
-        chain<T, KB, false><<<chain_grid(a), 64 * kChainWaves, 0, s>>>(a);
+        chain<T, KB, NW, false><<<chain_grid(a, NW), 64 * (NW + 4), 0, s>>>(a);
       return hip_check("kdelta chain launch");
     });
   });
@@ -1040,25 +1237,28 @@ extern "C" int kdelta_scan_bwd(const kdelta_problem* p, const void* d_o, const i
   const bool rows = p->B && p->N;
   if (rows && (!d_o || !do_strides || !saved || !dq || !dq_strides || !dk || !dk_strides || !dv || !dv_strides || !dg || !dbeta))
     return fail(KDECAY_EINVAL, "null pointer argument");
-  if (rows && ((do_strides[3] != 1 && p->Dv != 1) || (dq_strides[3] != 1 && p->Dk != 1) ||
-               (dk_strides[3] != 1 && p->Dk != 1) || (dv_strides[3] != 1 && p->Dv != 1)))
-    return fail(KDECAY_ELAYOUT, "channel (d) stride must be 1");
+  if (rows) {
+    const struct {
+      const void* p;
+      const int64_t* strides;
+      const char* name;
+    } all[] = {{d_o, do_strides, "d_o"}, {dq, dq_strides, "dq"}, {dk, dk_strides, "dk"}, {dv, dv_strides, "dv"}};
+    for (const auto& x : all)
+      if (const int rc = check_rows(x.p, x.strides, p->dtype, x.name)) return rc;
+  }
   if (workspace_bytes < kdelta_scan_bwd_workspace_bytes(p) || (!workspace && rows) || ((uintptr_t)workspace & 15))
     return fail(KDECAY_EWORKSPACE, "backward workspace of %zu bytes missing, small or not 16-byte aligned",
                 kdelta_scan_bwd_workspace_bytes(p));
   if ((uintptr_t)saved & 15) return fail(KDECAY_ELAYOUT, "saved is not 16-byte aligned");
-  Args a = args_of(p, workspace);
+  Args a = args_of(p, workspace, true);
   a.states = const_cast<float*>(saved);
-  a.us = a.states + (size_t)a.tiles * a.H * a.Dk * a.Dv;
+  a.us = a.states + (size_t)a.tiles * a.H * a.groups * 2 * ((a.Dk + 31) / 32) * 256;
   a.d_o = d_o, a.d_final = d_final, a.d_init = d_init, a.dq = dq, a.dk = dk, a.dv = dv, a.dg = dg, a.dbeta = dbeta;
   if (rows) {
     a.dob = do_strides[0], a.doh = do_strides[1], a.don = do_strides[2];
     a.dqb = dq_strides[0], a.dqh = dq_strides[1], a.dqn = dq_strides[2];
     a.dkb = dk_strides[0], a.dkh = dk_strides[1], a.dkn = dk_strides[2];
     a.dvb = dv_strides[0], a.dvh = dv_strides[1], a.dvn = dv_strides[2];
-    a.vec_do = aligned4(d_o, do_strides, p->dtype);
-    a.vec_dq = aligned4(dq, dq_strides, p->dtype);
-    a.vec_dk = aligned4(dk, dk_strides, p->dtype);
   }
   const hipStream_t s = (hipStream_t)stream;
   return by_type(p->dtype, [&](auto* t) {
@@ -1069,7 +1269,7 @@ extern "C" int kdelta_scan_bwd(const kdelta_problem* p, const void* d_o, const i
         prep<T, KB, true><<<dim3((unsigned)a.tiles, a.H), 256, 0, s>>>(a);
         if (const int rc = hip_check("kdelta prep launch")) return rc;
       }
-      chain_back<T, KB><<<chain_grid(a), 64 * kChainWaves, 0, s>>>(a);
+      chain_back<T, KB><<<chain_grid(a, kBackWaves), 64 * kBackWaves, 0, s>>>(a);
       if (const int rc = hip_check("kdelta chain_back launch")) return rc;
       if (!rows) return 0;
       grads<T, KB><<<dim3((unsigned)a.tiles, a.Hk), 256, 0, s>>>(a);

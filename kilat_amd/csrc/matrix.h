@@ -89,47 +89,58 @@ inline constexpr int kInputTerms<__bf16> = 1;
 template <>
 inline constexpr int kInputTerms<_Float16> = 2;
 
-// p[0..3] as floats, zero from element n on.  vec: p is aligned to four elements.
+// Rows are whole fours of elements, aligned to four (the hosts' checks and copies see to it),
+// so four elements are all there or none of them is: n, the elements left, is 0 or
+// less, or 4 or more.
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p, int64_t n, bool vec) {
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (vec && n >= 4) {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    const T4 x = *reinterpret_cast<const T4*>(p);
+using Raw4 = T __attribute__((ext_vector_type(4)));
+
+// Loads that are to stay in flight: no branch that depends on the lane, and no conversion,
+// until the values are used.  base itself is read where there is nothing to read.
+template <typename T>
+__device__ __forceinline__ Raw4<T> fetch4(const T* base, int64_t at, int n) {
+  return *reinterpret_cast<const Raw4<T>*>(base + (n > 0 ? at : 0));
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 fetched(Raw4<T> x, int n) {
+  f32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (float)x[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) r[i] = (float)p[i];
-  }
+  for (int i = 0; i < 4; ++i) r[i] = n > 0 ? (float)x[i] : 0.f;
   return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T* p, f32x4 x, int64_t n, bool vec) {
-  if (vec && n >= 4) {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T4 y;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = (T)x[i];
-    *reinterpret_cast<T4*>(p) = y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = (T)x[i];
-  }
+__device__ __forceinline__ f32x4 load4(const T* base, int64_t at, int n) {
+  return fetched<T>(fetch4(base, at, n), n);
 }
 
-// One lane's eight values of a row: inner indices k0 + 4g + i and k0 + 16 + 4g + i, zero
-// from index `width` on.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int k0, int g, int width, bool vec, float (&x)[8]) {
-  const int a = k0 + 4 * g;
-  const f32x4 lo = load4(row + a, width - a, vec), hi = load4(row + a + 16, width - a - 16, vec);
+__device__ __forceinline__ void store4(T* p, f32x4 x) {
+  Raw4<T> y;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
+  for (int i = 0; i < 4; ++i) y[i] = (T)x[i];
+  *reinterpret_cast<Raw4<T>*>(p) = y;
 }
+
+// Results of matrix instructions are written up to 16 passes after they issue, and nothing in
+// the hardware holds back an instruction that reads or overwrites them earlier.  The
+// compiler keeps the distance inside a basic block only (measured: a loop-carried
+// accumulator copied at the head of the next block held its old value), so results
+// that are used, or whose registers are reused, behind a branch, barrier or loop end are settled
+// first.
+__device__ __forceinline__ void settle(f32x4& x) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(x)); }
+__device__ __forceinline__ void settle(f32x16& x) { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" : "+v"(x)); }
+template <typename V, int N>
+__device__ __forceinline__ void settle(V (&x)[N]) {
+#pragma unroll
+  for (int i = 1; i < N; ++i) asm volatile("" : "+v"(x[i]));
+  settle(x[0]);
+}
+
+// The wavefront's number in its workgroup, known to the compiler to be one for all its
+// lanes: branches on it are scalar, and barriers behind them are reached by whole wavefronts.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
 // Sum over the four lane groups (lanes l, l^16, l^32, l^48).
 __device__ __forceinline__ float group_sum(float x) {
@@ -207,6 +218,14 @@ __device__ __forceinline__ void zero_outside(const int32_t* cu, int64_t sequence
   for (int64_t r = tile * C; r < end; ++r)
     if (r < lo || r >= hi)
       for (int d = thread; d < width; d += threads) x[r * row_stride + d] = (T)0.f;
+}
+
+// The hosts' check of one tensor of rows: channels adjacent, every row aligned to four elements.
+inline int check_rows(const void* p, const int64_t* strides, int dtype, const char* name) {
+  if (strides[3] != 1) return fail(KDECAY_ELAYOUT, "%s: channel (d) stride must be 1", name);
+  if (((uintptr_t)p & (dtype == KDECAY_F32 ? 15u : 7u)) || strides[0] % 4 || strides[1] % 4 || strides[2] % 4)
+    return fail(KDECAY_ELAYOUT, "%s: base and strides must be multiples of four elements", name);
+  return 0;
 }
 
 }  // namespace kd

@@ -8,6 +8,8 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/torch.h>
 
+#include <array>
+
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
@@ -57,17 +59,36 @@ void check_float(const Tensor& t, const Tensor& q, const char* name) {
 // `t` as float32 (recorded by autograd where it converts).
 Tensor as_float(const Tensor& t) { return t.to(at::kFloat).resolve_neg(); }
 
-// `t` as the kernels read it: channels adjacent, its memory holding its values.
+// Whether the kernels read (and write) `t` as it lies: channels adjacent, every row aligned to
+// four elements.  For head dims that are multiples of 4.
+bool rows_ok(const Tensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % (4 * t.element_size()) || t.stride(3) != 1) return false;
+  for (int64_t k = 0; k < 3; ++k)
+    if (t.size(k) > 1 && t.stride(k) % 4) return false;
+  return true;
+}
+
+// `t` as the kernels read it, its memory holding its values.  (A contiguous tensor off the
+// alignment is its own contiguous().)
 Tensor as_rows(const Tensor& t) {
   const Tensor r = t.resolve_neg();
-  return r.size(-1) == 1 || r.stride(-1) == 1 ? r : r.contiguous();
+  return rows_ok(r) ? r : r.clone(at::MemoryFormat::Contiguous);
 }
 
 // A new tensor of `like`'s shape and, as far as the kernels write it, its layout.
 Tensor new_like(const Tensor& like) {
   Tensor r = at::empty_like(like);
-  if (r.size(-1) != 1 && r.stride(-1) != 1) r = at::empty(like.sizes(), like.options());
+  if (!rows_ok(r)) r = at::empty(like.sizes(), like.options());
   return r;
+}
+
+// Channels (of dimension `dim`) padded with zeros to a multiple of 4.
+Tensor pad4(const Tensor& t, int64_t dim) {
+  const int64_t n = t.size(dim);
+  if (n % 4 == 0) return t;
+  std::vector<int64_t> pad(2 * (t.dim() - dim), 0);
+  pad.back() = 4 - n % 4;
+  return at::constant_pad_nd(t, pad, 0);
 }
 
 // cu_seqlens, or an undefined tensor.
@@ -96,7 +117,13 @@ const void* cptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nu
 float* fptr(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
 
 void copy_strides(int64_t* to, const Tensor& t) {
-  for (int64_t k = 0; k < t.dim(); ++k) to[k] = t.stride(k);
+  for (int64_t k = 0; k < t.dim(); ++k) to[k] = k < 3 && t.size(k) == 1 ? 0 : t.stride(k);
+}
+
+std::array<int64_t, 4> strides(const Tensor& t) {
+  std::array<int64_t, 4> r;
+  copy_strides(r.data(), t);
+  return r;
 }
 
 // ---------------------------------------------------------------------------
@@ -135,7 +162,7 @@ Scanned delta_forward(const kdelta_problem& p, const Tensor& v, bool want_final,
   if (save) r.saved = at::empty({static_cast<int64_t>(kdelta_scan_saved_floats(&p))}, f32);
   const size_t n = kdelta_scan_workspace_bytes(&p);
   const Tensor ws = bytes_on(v, n);
-  check_rc(kdelta_scan_fwd(&p, r.o.data_ptr(), r.o.strides().data(), fptr(r.final), save && r.saved.numel() ? fptr(r.saved) : nullptr,
+  check_rc(kdelta_scan_fwd(&p, r.o.data_ptr(), strides(r.o).data(), fptr(r.final), save && r.saved.numel() ? fptr(r.saved) : nullptr,
                            ws.data_ptr(), n, stream_of(v)),
            "kdelta_scan_fwd");
   return r;
@@ -163,7 +190,6 @@ struct DeltaNode : torch::autograd::Function<DeltaNode> {
     const kdelta_problem p = problem(q, k, v, g, beta, cu, init, ctx->saved_data["scale"].toDouble());
     const c10::DeviceGuard guard(v.device());
     const Tensor d_o = grads[0].defined() ? as_rows(grads[0].to(v.scalar_type())) : at::zeros_like(v);
-    const Tensor d_o4 = d_o.size(-1) == 1 || d_o.stride(-1) == 1 ? d_o : d_o.contiguous();
     const Tensor d_final = grads[1].defined() ? grads[1].to(at::kFloat).resolve_neg().contiguous() : Tensor();
     const auto f32 = v.options().dtype(at::kFloat);
     const Tensor dq = new_like(q), dk = new_like(k), dv = new_like(v);
@@ -171,8 +197,8 @@ struct DeltaNode : torch::autograd::Function<DeltaNode> {
     const Tensor d_init = init.defined() ? at::empty(init.sizes(), f32) : Tensor();
     const size_t n = kdelta_scan_bwd_workspace_bytes(&p);
     const Tensor ws = bytes_on(v, n);
-    check_rc(kdelta_scan_bwd(&p, d_o4.const_data_ptr(), d_o4.strides().data(), fptr(d_final), fptr(states), dq.data_ptr(),
-                             dq.strides().data(), dk.data_ptr(), dk.strides().data(), dv.data_ptr(), dv.strides().data(),
+    check_rc(kdelta_scan_bwd(&p, d_o.const_data_ptr(), strides(d_o).data(), fptr(d_final), fptr(states), dq.data_ptr(),
+                             strides(dq).data(), dk.data_ptr(), strides(dk).data(), dv.data_ptr(), strides(dv).data(),
                              fptr(dg), fptr(dbeta), fptr(d_init), ws.data_ptr(), n, stream_of(v)),
              "kdelta_scan_bwd");
     return {dq, dk, dv, dg, dbeta, d_init, Tensor(), Tensor()};
@@ -212,9 +238,9 @@ py::object delta_scan(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   require_hip(q_in, "q");
   cu = as_cu(cu);
   const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(Dk));
-  Tensor q = as_rows(q_in), k = as_rows(k_in), v = as_rows(v_in);
+  Tensor q = as_rows(pad4(q_in, 3)), k = as_rows(pad4(k_in, 3)), v = as_rows(pad4(v_in, 3));
   Tensor g = as_float(g_in), beta = as_float(beta_in);
-  if (init.defined()) init = as_float(init).contiguous();
+  if (init.defined()) init = pad4(pad4(as_float(init), 3), 2).contiguous();
   Tensor o, final;
   {
     py::gil_scoped_release nogil;
@@ -228,6 +254,8 @@ py::object delta_scan(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
       const Scanned r = delta_forward(problem(q, k, v, g, beta, cu, init, scale), v, want_final, false);
       o = r.o, final = r.final;
     }
+    if (Dv % 4) o = at::empty_like(v_in).copy_(o.narrow(3, 0, Dv));
+    if (want_final && (Dk % 4 || Dv % 4)) final = final.narrow(2, 0, Dk).narrow(3, 0, Dv).contiguous();
   }
   return want_final ? py::object(py::make_tuple(o, final)) : py::cast(o);
 }
@@ -333,20 +361,24 @@ Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, std
   TORCH_CHECK(!grad_wanted({&q_in, &k_in, &v_in}),
               "kilat_amd: causal_attention has no backward; call it under torch.no_grad()");
   at::AutoDispatchBelowADInplaceOrView below;  // new buffers only: nothing to record
-  const Tensor q = as_rows(q_in), k = as_rows(k_in), v = as_rows(v_in), cu = as_cu(cu_any);
+  const Tensor q = as_rows(pad4(q_in, 3)), k = as_rows(pad4(k_in, 3)), v = as_rows(pad4(v_in, 3)), cu = as_cu(cu_any);
   const c10::DeviceGuard guard(q.device());
   // Laid out like q: rows of all heads together where q's are.
-  const bool tokens = H > 1 && N > 1 && q.stride(1) < q.stride(2);
-  const Tensor o = tokens ? at::empty({B, N, H, Dv}, q.options()).transpose(1, 2) : at::empty({B, H, N, Dv}, q.options());
+  const bool tokens = H > 1 && N > 1 && q_in.stride(1) < q_in.stride(2);
+  const auto empty = [&](int64_t D) {
+    return tokens ? at::empty({B, N, H, D}, q.options()).transpose(1, 2) : at::empty({B, H, N, D}, q.options());
+  };
+  const Tensor o = empty(v.size(3));
   kattn_problem p = {};
   p.q = q.const_data_ptr(), p.k = k.const_data_ptr(), p.v = v.const_data_ptr();
   p.cu_seqlens = static_cast<const int32_t*>(cptr(cu));
   copy_strides(p.q_strides, q), copy_strides(p.k_strides, k), copy_strides(p.v_strides, v);
-  p.B = B, p.Hk = Hk, p.H = H, p.N = N, p.Dk = Dk, p.Dv = Dv;
+  p.B = B, p.Hk = Hk, p.H = H, p.N = N, p.Dk = q.size(3), p.Dv = v.size(3);
   p.sequences = cu.defined() ? cu.numel() - 1 : B;
   p.scale = static_cast<float>(scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(Dk)));
   p.dtype = code_of(q, "q");
-  check_rc(kattn_fwd(&p, o.data_ptr(), o.strides().data(), stream_of(q)), "kattn_fwd");
+  check_rc(kattn_fwd(&p, o.data_ptr(), strides(o).data(), stream_of(q)), "kattn_fwd");
+  if (Dv % 4) return empty(Dv).copy_(o.narrow(3, 0, Dv));
   return o;
 }
 
