@@ -26,8 +26,8 @@ extern "C" {
 
 /*
  * q [B,H,N,Dk], k [B,Hk,N,Dk], v [B,Hk,N,Dv], with strides for their four dimensions, as
- * kdelta.h asks of rows: the last is 1, the others, the bases and the head dims multiples of
- * four elements.  cu_seqlens and sequences: as in
+ * kdelta.h asks of rows: the last is 1, the others and the bases are multiples of 16
+ * bytes, and the head dims of 8.  cu_seqlens and sequences: as in
  * kdelta.h (kdelta_problem).
  */
 typedef struct kattn_problem {

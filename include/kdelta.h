@@ -33,8 +33,8 @@ extern "C" {
 
 /*
  * One problem.  Tensors are [B, heads, N, D] with strides for their four
- * dimensions: the last is 1, the others and the base are multiples of four elements
- * (strides of dimensions of size 1 too: give 0), and Dk and Dv are multiples of 4
+ * dimensions: the last is 1, the others and the base are multiples of 16 bytes
+ * (strides of dimensions of size 1 too: give 0), and Dk and Dv are multiples of 8
  * (KDECAY_ELAYOUT, KDECAY_ESHAPE otherwise; zero channels of q and k change nothing).  g and beta are float32
  * [B, H, N] with three strides.  H is a multiple of Hk.
  *

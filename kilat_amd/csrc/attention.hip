@@ -305,8 +305,8 @@ int check(const kattn_problem* p, const void* o, const int64_t* o_strides) {
   if (!p->cu_seqlens && p->sequences != p->B) return fail(KDECAY_EINVAL, "sequences must be B without cu_seqlens");
   if (p->sequences > 0x7fffffff || tiles_of<32>(p) > 0x7fffffff)
     return fail(KDECAY_ESHAPE, "too many sequences or rows");
-  if (p->Dk % 4 || p->Dv % 4)
-    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not multiples of 4", (long long)p->Dk, (long long)p->Dv);
+  if (p->Dk % 8 || p->Dv % 8)
+    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not multiples of 8", (long long)p->Dk, (long long)p->Dv);
   if (!p->B || !p->N) return 0;
   if (!p->q || !p->k || !p->v || !o || !o_strides) return fail(KDECAY_EINVAL, "null pointer argument");
   if (const int rc = check_rows(p->q, p->q_strides, p->dtype, "q")) return rc;

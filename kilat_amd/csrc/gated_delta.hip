@@ -34,7 +34,7 @@ constexpr int kOutTerms = sizeof(T) == 4 ? 3 : 2;
 template <typename T>
 constexpr int kOutOrder = sizeof(T) == 4 ? 2 : 1;
 
-// Per token of a chunk, floats.
+// Per token of a chunk, floats: b e^G, b, e^G, e^(G_64 - G), and G log2(e) as the sum of two.
 enum Vec { V_BG, V_BETA, V_SINCE, V_LEFT, V_G, V_GLOW, V_COUNT };
 
 struct Args {
@@ -47,9 +47,8 @@ struct Args {
   int Hk, H, Dk, Dv, group, groups;  // value heads of a key head; 16-column groups of Dv
   float scale;
   // scratch, by tile and head
-  float* inv;      // [tiles][H][kTri][2][64][4]: T as operand tiles
   __bf16* keys;    // backward: [tiles][Hk][3][4 KB][NI][kFrag]: K, its transpose, Q's transpose
-  __bf16* tris;    // backward: [tiles][H][kTri * 2 * NX][kFrag]: T's transpose and P's
+  __bf16* tris;    // [tiles][H][kTri * NX][kFrag]: T (backward: [kTri * 2 * NX], T's transpose and P's)
   float* vecs;     // [tiles][H][V_COUNT][C]
   float* states;   // saved: [tiles][H][16-column groups][2 KB][64][4], S at the chunk's start as it lies in registers
   float* us;       // saved: [tiles][H][16-column groups][4][64][4]: u
@@ -68,13 +67,19 @@ struct Args {
   float *dg, *dbeta;
 };
 
+// The channel of k that row r of the 16-row tile dt of a state (or of K transposed) is. In steps of 32,
+// the order in which lane group g's eight inner indices of an operand, tiles 2kb and 2kb+1 of
+// a state, are the channels 8g..8g+7: an operand of k's rows is loaded as they lie.
+__host__ __device__ constexpr int channel(int dt, int r) { return 32 * (dt >> 1) + 8 * (r >> 2) + 4 * (dt & 1) + (r & 3); }
+
 // Where a tile's operands are.
 template <int KB, int NI>
 __device__ __forceinline__ __bf16* key_tiles(const Args& a, int64_t tile, int hk) {
   return a.keys + ((tile * a.Hk + hk) * 3) * (int64_t)(4 * KB * NI * kFrag);
 }
+template <bool BWD>
 __device__ __forceinline__ __bf16* tri_tiles(const Args& a, int64_t tile, int h) {
-  return a.tris + (tile * a.H + h) * (int64_t)(kTri * 2 * NX * kFrag);
+  return a.tris + (tile * a.H + h) * (int64_t)(kTri * (BWD ? 2 : 1) * NX * kFrag);
 }
 __device__ __forceinline__ float* vec_of(const Args& a, int64_t tile, int h) {
   return a.vecs + (tile * a.H + h) * (int64_t)(V_COUNT * C);
@@ -93,12 +98,38 @@ __device__ __forceinline__ void store_terms(__bf16* p, int lane, const Terms<N>&
   for (int n = 0; n < N; ++n) *reinterpret_cast<bf16x8*>(p + n * kFrag + lane * 8) = x.t[n];
 }
 
-// Tile f of the transpose of a chunk's rows, from their tiles in LDS (rows are channels
-// 16 (f / 2) + lane % 16, inner indices tokens of half f % 2).
+// The terms of one lane's fetched eight of a row, of which there are n (0 or less, or 8).
+template <typename T>
+__device__ __forceinline__ Terms<kInputTerms<T>> terms_of(Raw8<T> x, int n) {
+  if constexpr (kInputTerms<T> == 1) {
+    const uint4 y = __builtin_bit_cast(uint4, x);
+    Terms<1> r;
+    r.t[0] = __builtin_bit_cast(bf16x8, make_uint4(n > 0 ? y.x : 0u, n > 0 ? y.y : 0u, n > 0 ? y.z : 0u, n > 0 ? y.w : 0u));
+    return r;
+  } else {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = n > 0 ? (float)x[i] : 0.f;
+    return split<kInputTerms<T>>(y);
+  }
+}
+
+// A product with one of these picks 16 of an operand's 32 inner indices as they are: rows that lie
+// along lanes come out along registers, so it transposes a tile.  This one picks index `inner` in
+// the result's column m.
+__device__ __forceinline__ bf16x8 selector(int inner, int g) {
+  bf16x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (__bf16)(8 * g + i == inner ? 1.f : 0.f);
+  return r;
+}
+
+// Tile f of the transpose of a chunk's rows, from their tiles in LDS (rows are channels, inner
+// indices tokens of half f % 2).
 template <int KB, int NI>
 __device__ __forceinline__ Terms<NI> transposed(const __bf16* tiles, int f, int lane) {
-  const int d = 16 * (f / 2) + (lane & 15), t0 = 32 * (f & 1) + 4 * (lane >> 4);
-  const int src = (d / 32) * NI * kFrag + (d & 3) + ((d >> 4) & 1) * 4, sl = 16 * ((d >> 2) & 3);
+  const int d = channel(f / 2, lane & 15), t0 = 32 * (f & 1) + 4 * (lane >> 4);
+  const int src = (d / 32) * NI * kFrag + (d & 7), sl = 16 * ((d >> 3) & 3);
   Terms<NI> r;
 #pragma unroll
   for (int j = 0; j < NI; ++j)
@@ -117,6 +148,10 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// 2^x, by the instruction: x is a difference of two sums of log decays, exact to 2^-24 of
+// itself, so what is at most 1 is off by 2^-24 x 2^x, less than its last digit.
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // e^x for a difference of sums of log decays (positive for a growing state only).
 __device__ __forceinline__ float fade(double x) {
   const float hi = (float)x, e = expf(hi);
@@ -127,8 +162,7 @@ __device__ __forceinline__ float fade(double x) {
 // prep: T of one chunk and value head (BWD: what the backward's products take)
 // --------------------------------------------------------------------------
 // Grid (tiles, H), four wavefronts; wavefront w has tokens 16w..16w+15 of the chunk.
-// Forward: T, as operand tiles in 32 bits.  BWD: T and P transposed, K, K transposed and
-// Q transposed, as operand tiles of terms.
+// Operand tiles of terms, forward: T.  BWD: T and P transposed, K, K transposed and Q transposed.
 //
 // log decays are added up in 64 bits: the sums over a chunk can be far larger than
 // the differences that count.  One below -128 is taken as -128: e^-128 is 0 in 32 bits,
@@ -157,15 +191,13 @@ __global__ __launch_bounds__(256) void prep(Args a) {
   const int t = 16 * w + m;
   const T* kbase = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + row0 * a.kn;
   const T* qbase = (const T*)a.q + at.rows.batch * a.qb + hk * a.qh + row0 * a.qn;
-  Raw4<T> kr[KB][2], qr[BWD ? KB : 1][2];
+  Raw8<T> kr[KB], qr[BWD ? KB : 1];
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int d = 32 * kb + 16 * x + 4 * g, left = t < n ? a.Dk - d : 0;
-      kr[kb][x] = fetch4(kbase, t * a.kn + d, left);
-      if (BWD) qr[BWD ? kb : 0][x] = fetch4(qbase, t * a.qn + d, left);
-    }
+  for (int kb = 0; kb < KB; ++kb) {
+    const int d = 32 * kb + 8 * g, left = t < n ? a.Dk - d : 0;
+    kr[kb] = fetch8(kbase, t * a.kn + d, left);
+    if (BWD) qr[BWD ? kb : 0] = fetch8(qbase, t * a.qn + d, left);
+  }
   if (w == 0) {
     const bool in = lane < n;
     double G = 0.;
@@ -189,18 +221,17 @@ __global__ __launch_bounds__(256) void prep(Args a) {
     vec[V_BETA * C + lane] = b;
     vec[V_SINCE * C + lane] = since;
     vec[V_LEFT * C + lane] = fade(all - G);
-    vec[V_G * C + lane] = (float)G;
-    vec[V_GLOW * C + lane] = (float)(G - (double)(float)G);
+    const double G2 = G * 1.4426950408889634074;
+    vec[V_G * C + lane] = (float)G2;
+    vec[V_GLOW * C + lane] = (float)(G2 - (double)(float)G2);
   }
   Terms<NI> kt[KB];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    const int d = 32 * kb + 4 * g, left = t < n ? a.Dk - d : 0;
-    kt[kb] = split<NI>(fetched<T>(kr[kb][0], left), fetched<T>(kr[kb][1], left - 16));
+    const int left = t < n ? a.Dk - 32 * kb - 8 * g : 0;
+    kt[kb] = terms_of<T>(kr[kb], left);
     store_terms<NI>(kq[0] + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
-    if constexpr (BWD)
-      store_terms<NI>(kq[1] + (w * KB + kb) * NI * kFrag, lane,
-                      split<NI>(fetched<T>(qr[kb][0], left), fetched<T>(qr[kb][1], left - 16)));
+    if constexpr (BWD) store_terms<NI>(kq[1] + (w * KB + kb) * NI * kFrag, lane, terms_of<T>(qr[kb], left));
   }
   __syncthreads();
   if constexpr (BWD) {
@@ -232,7 +263,7 @@ __global__ __launch_bounds__(256) void prep(Args a) {
     }
   }
   if constexpr (BWD) {  // P transposed: rows j of this wavefront
-    __bf16* tri = tri_tiles(a, tile, h);
+    __bf16* tri = tri_tiles<true>(a, tile, h);
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
       if (kb2 < w / 2) continue;
@@ -310,13 +341,8 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       const int o = 32 * kb2 + 4 * g + (i & 3) + 16 * (i >> 2);
       x[i >> 2][i & 3] = BWD ? Ts[o * LD + t] : Ts[t * LD + o];
     }
-    if constexpr (BWD) {
-      store_terms<NX>(tri_tiles(a, tile, h) + tri_upper(w, kb2) * NX * kFrag, lane, split<NX>(x[0], x[1]));
-    } else {
-      float* out = a.inv + ((tile * a.H + h) * kTri + tri_lower(w, kb2)) * (int64_t)kFrag + lane * 4;
-      *reinterpret_cast<f32x4*>(out) = x[0];
-      *reinterpret_cast<f32x4*>(out + 256) = x[1];
-    }
+    const int f = BWD ? tri_upper(w, kb2) : tri_lower(w, kb2);
+    store_terms<NX>(tri_tiles<BWD>(a, tile, h) + f * NX * kFrag, lane, split<NX>(x[0], x[1]));
   }
 }
 
@@ -337,10 +363,10 @@ __device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, 
     float x = 0.f;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      const f32x4 k = load4(krow, 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g);
+      const f32x4 k = load4(krow, channel(dt, 4 * g), a.Dk - channel(dt, 4 * g));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (16 * dt + 4 * g + i < a.Dk) {
+        if (channel(dt, 4 * g) < a.Dk) {
           S[dt][i] *= dec;
           x = fmaf(k[i], S[dt][i], x);
         }
@@ -352,11 +378,11 @@ __device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, 
     float o = 0.f;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      const f32x4 k = load4(krow, 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g);
-      const f32x4 q = load4(qrow, 16 * dt + 4 * g, a.Dk - 16 * dt - 4 * g);
+      const f32x4 k = load4(krow, channel(dt, 4 * g), a.Dk - channel(dt, 4 * g));
+      const f32x4 q = load4(qrow, channel(dt, 4 * g), a.Dk - channel(dt, 4 * g));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (16 * dt + 4 * g + i < a.Dk) {
+        if (channel(dt, 4 * g) < a.Dk) {
           S[dt][i] = fmaf(k[i], u, S[dt][i]);
           o = fmaf(q[i], S[dt][i], o);
         }
@@ -383,7 +409,7 @@ template <typename T, int KB, int NW, bool SAVE>
 __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>, ORD = kOutOrder<T>;
   __shared__ __bf16 Kf[4 * KB * NI * kFrag], Kt[4 * KB * NI * kFrag], Tf[kTri * NX * kFrag];
-  __shared__ T Vf[NW * 4 * 256];
+  __shared__ float Vf[NW * 4 * 256];
   __shared__ __bf16 Sf[NW * KB * NO * kFrag], Uf[NW * 2 * NO * kFrag];
   __shared__ float vecs[2][V_COUNT * C];
   __shared__ int by_token[NW];
@@ -401,7 +427,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int d = 16 * dt + 4 * g + i;
+        const int d = channel(dt, 4 * g + i);
         S[dt][i] = a.init && in && d < a.Dk ? a.init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
       }
     if (nch) lds_barrier();
@@ -424,10 +450,13 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
             *reinterpret_cast<bf16x8*>(Sf + ((wave * KB + kb) * NO + j) * kFrag + lane * 8) = s[kb].t[j];
         }
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          X[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int mt = 0; mt < 4; ++mt) X[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) X[mt] = product<2>(load_terms<NI>(Kf + (mt * KB + kb) * NI * kFrag, lane), s[kb], X[mt]);
+        for (int kb = 0; kb < KB; ++kb) {
+          Terms<NI> k[4];
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) k[mt] = load_terms<NI>(Kf + (mt * KB + kb) * NI * kFrag, lane);
+          products<2>(k, s[kb], X);
         }
         settle(X);
       }
@@ -437,25 +466,31 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
         for (int mt = 0; mt < 4; ++mt) {
           const f32x4 bg = *reinterpret_cast<const f32x4*>(vec + V_BG * C + 16 * mt + 4 * g);
           const f32x4 b = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * mt + 4 * g);
-          const f32x4 v = load4(Vf, (wave * 4 + mt) * 256 + lane * 4, 4);
-          X[mt] = b * v - bg * X[mt];
+          const f32x4 v = *reinterpret_cast<const f32x4*>(Vf + (wave * 4 + mt) * 256 + lane * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) X[mt][i] = fmaf(-bg[i], X[mt][i], b[i] * v[i]);
         }
         const Terms<NX> r[2] = {split<NX>(X[0], X[1]), split<NX>(X[2], X[3])};
         f32x4 U[4];
         float odd = 0.f;
+        {
+          Terms<NX> x[4], y[2];
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          f32x4 x = {0.f, 0.f, 0.f, 0.f};
+          for (int mt = 0; mt < 4; ++mt) {
+            U[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            x[mt] = load_terms<NX>(Tf + tri_lower(mt, 0) * NX * kFrag, lane);
+          }
+          products<2>(x, r[0], U);
 #pragma unroll
-          for (int kb = 0; kb <= mt / 2; ++kb) x = product<2>(load_terms<NX>(Tf + tri_lower(mt, kb) * NX * kFrag, lane), r[kb], x);
-          U[mt] = x;
+          for (int mt = 2; mt < 4; ++mt) y[mt - 2] = load_terms<NX>(Tf + tri_lower(mt, 1) * NX * kFrag, lane);
+          products<2>(y, r[1], U + 2);
         }
         settle(U);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) odd += 0.f * U[mt][i];
-        const bool slow = __any(odd != 0.f);  // NaN: something is not finite
+          for (int i = 0; i < 4; ++i) odd += U[mt][i];
+        const bool slow = __any(!(fabsf(odd) <= 3.402823466e38f));  // something is not finite
         if (lane == 0) by_token[wave] = slow;
         if (slow) {
           chunk_by_token<T, KB, SAVE>(a, rows, rows.first + c * C, rows.n - c * C < C ? (int)(rows.n - c * C) : C, h, col,
@@ -475,10 +510,13 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
           for (int mt = 0; mt < 4; ++mt) U[mt] *= *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
           const Terms<NX> ul[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
 #pragma unroll
-          for (int dt = 0; dt < 2 * KB; ++dt) {
-            S[dt] *= whole;
+          for (int dt = 0; dt < 2 * KB; ++dt) S[dt] *= whole;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) S[dt] = product<2>(load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane), ul[kb], S[dt]);
+          for (int kb = 0; kb < 2; ++kb) {
+            Terms<NI> k[2 * KB];
+#pragma unroll
+            for (int dt = 0; dt < 2 * KB; ++dt) k[dt] = load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane);
+            products<2>(k, ul[kb], S);
           }
           settle(S);
         }
@@ -490,7 +528,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
       for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int d = 16 * dt + 4 * g + i;
+          const int d = channel(dt, 4 * g + i);
           if (in && d < a.Dk) a.final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
         }
     }
@@ -503,128 +541,149 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   const T* qbase = (const T*)a.q + rows.batch * a.qb + hk * a.qh + rows.first * a.qn;
   const T* vbase = (const T*)a.v + rows.batch * a.vb + h * a.vh + rows.first * a.vn;
   T* obase = (T*)a.o + rows.batch * a.ob + h * a.oh + rows.first * a.on;
-  // V: four lanes per token, 4 NW columns each; T: three tile halves per wavefront.
-  const int vt = 16 * w + (lane >> 2), vc = (lane & 3) * 4 * NW;
-  Raw4<T> kr[KB][2], qr[KB][2], vr[NW];
-  f32x4 tr[3], er;
-  const auto fetch = [&](int64_t c) {
-    const int64_t row = c * C + t;
-    const int dk = row < rows.n ? a.Dk : 0;
+  constexpr int VB = (NW + 1) / 2;             // 32-column blocks of V
+  constexpr int TP = (kTri * NX + 3) / 4;      // planes of T per feeder: w, w + 4, ...
+  const T *kp = kbase + t * a.kn + 8 * g, *qp = qbase + t * a.qn + 8 * g, *vp = vbase + t * a.vn + col0 + 8 * g;
+  const __bf16* ip = tri_tiles<false>(a, tile0, h) + w * kFrag + lane * 8;
+  const float* ep = vec_of(a, tile0, h) + (ft % (V_COUNT * C / 4)) * 4;
+  Raw8<T> kr[KB], qr[KB], vr[VB];
+  bf16x8 tr[TP];
+  f32x4 er;
+  int left = rows.n < t ? 0 : rows.n - t < 0x7fffffff ? (int)(rows.n - t) : 0x7fffffff;  // rows from this lane's on
+  const auto fetch = [&]() {  // the next chunk's
+    const int dk = left > 0 ? a.Dk - 8 * g : 0, dv = left > 0 ? a.Dv - col0 - 8 * g : 0;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < KB; ++kb) {
+      kr[kb] = *reinterpret_cast<const Raw8<T>*>(32 * kb < dk ? kp + 32 * kb : kbase);
+      qr[kb] = *reinterpret_cast<const Raw8<T>*>(32 * kb < dk ? qp + 32 * kb : qbase);
+    }
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int d = 32 * kb + 16 * x + 4 * g;
-        kr[kb][x] = fetch4(kbase, row * a.kn + d, dk - d);
-        qr[kb][x] = fetch4(qbase, row * a.qn + d, dk - d);
-      }
-    const int64_t vrow = c * C + vt;
-    const int dv = vrow < rows.n ? a.Dv - col0 - vc : 0;
+    for (int b = 0; b < VB; ++b) vr[b] = *reinterpret_cast<const Raw8<T>*>(32 * b < dv ? vp + 32 * b : vbase);
 #pragma unroll
-    for (int x = 0; x < NW; ++x) vr[x] = fetch4(vbase, vrow * a.vn + col0 + vc + 4 * x, dv - 4 * x);
-    const float* inv = a.inv + ((tile0 + c) * a.H + h) * (int64_t)(kTri * kFrag);
-#pragma unroll
-    for (int x = 0; x < 3; ++x) tr[x] = *reinterpret_cast<const f32x4*>(inv + (3 * w + x) * 256 + lane * 4);
-    er = *reinterpret_cast<const f32x4*>(vec_of(a, tile0 + c, h) + (ft % (V_COUNT * C / 4)) * 4);
+    for (int x = 0; x < TP; ++x)
+      if (4 * x + 4 <= kTri * NX || w + 4 * x < kTri * NX) tr[x] = *reinterpret_cast<const bf16x8*>(ip + 4 * x * kFrag);
+    er = *reinterpret_cast<const f32x4*>(ep);
+    kp += C * a.kn, qp += C * a.qn, vp += C * a.vn;
+    ip += a.H * (int64_t)(kTri * NX * kFrag), ep += a.H * (int64_t)(V_COUNT * C);
   };
-  // What the lane fetched of a row of K or Q of chunk c.
-  const auto row_terms = [&](const Raw4<T> (&x)[2], int kb, int64_t c) {
-    const int left = c * C + t < rows.n ? a.Dk - 32 * kb - 4 * g : 0;
-    return split<NI>(fetched<T>(x[0], left), fetched<T>(x[1], left - 16));
-  };
+  Terms<NI> kt[KB];
   const auto put_keys = [&](int64_t c) {
+    const int dk = left > 0 ? a.Dk - 8 * g : 0;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) store_terms<NI>(Kf + (w * KB + kb) * NI * kFrag, lane, row_terms(kr[kb], kb, c));
+    for (int kb = 0; kb < KB; ++kb) {
+      kt[kb] = terms_of<T>(kr[kb], dk - 32 * kb);
+      store_terms<NI>(Kf + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
+    }
     if (ft < V_COUNT * C / 4) *reinterpret_cast<f32x4*>(vecs[c & 1] + ft * 4) = er;
   };
-  fetch(0);
+  // Columns of a 32-channel block of K in the order of a state's rows, and of V in its own.
+  const bf16x8 ksel[2] = {selector(channel(0, m), g), selector(channel(1, m), g)};
+  const bf16x8 vsel[2] = {selector(m, g), selector(16 + m, g)};
+  fetch();
   put_keys(0);
   lds_barrier();
   Terms<NO> p[2];  // P of the last chunk: lane m = token i, inner indices j
   f32x4 O[NW];     // scale e^G S' q of it
   const auto write_out = [&](int64_t c) {
+    f32x4 y[NW];
 #pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      if (col0 + 16 * x >= a.Dv) continue;
-      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < NW; ++x) y[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        if (kb <= w / 2) {
-          y = product<ORD>(load_terms<NO>(Uf + (x * 2 + kb) * NO * kFrag, lane), p[kb], y);
-          settle(y);
-        }
-      if (c * C + t < rows.n && !by_token[x] && col0 + 16 * x + 4 * g < a.Dv)
-        store4(obase + (c * C + t) * a.on + col0 + 16 * x + 4 * g, O[x] + y);
+    for (int kb = 0; kb < 2; ++kb) {
+      Terms<NO> u[NW];
+#pragma unroll
+      for (int x = 0; x < NW; ++x) u[x] = load_terms<NO>(Uf + (x * 2 + kb) * NO * kFrag, lane);
+      products<ORD>(u, p[kb], y);
     }
+    settle(y);
+    T* row = obase + (c * C + t) * a.on + col0 + 4 * g;
+#pragma unroll
+    for (int x = 0; x < NW; ++x)
+      if (c * C + t < rows.n && col0 + 16 * x + 4 * g < a.Dv && !by_token[x]) store4(row + 16 * x, O[x] + y[x]);
   };
   for (int64_t c = 0; c < nch; ++c) {
     const float* vec = vecs[c & 1];
-    // T and V
 #pragma unroll
-    for (int x = 0; x < 3; ++x) {
-      const int f = 3 * w + x;
-      f32x4 y = tr[x];
+    for (int x = 0; x < TP; ++x)
+      if (4 * x + 4 <= kTri * NX || w + 4 * x < kTri * NX)
+        *reinterpret_cast<bf16x8*>(Tf + (w + 4 * x) * kFrag + lane * 8) = tr[x];
+    // K and V transposed, q
 #pragma unroll
-      for (int j = 0; j < NX; ++j) {
-        bf16x4 e;
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x4 y[2 * NI];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = j + 1 < NX ? (__bf16)upper_half(y[i]) : (__bf16)y[i];
-          if (j + 1 < NX) y[i] -= upper_half(y[i]);
-        }
-        *reinterpret_cast<bf16x4*>(Tf + ((f >> 1) * NX + j) * kFrag + lane * 8 + 4 * (f & 1)) = e;
+      for (int x = 0; x < 2 * NI; ++x) y[x] = mfma(kt[kb].t[x % NI], ksel[x / NI], f32x4{0.f, 0.f, 0.f, 0.f});
+      settle(y);
+#pragma unroll
+      for (int x = 0; x < 2 * NI; ++x) {
+        const u32x2 r = {upper_halves(y[x][0], y[x][1]), upper_halves(y[x][2], y[x][3])};
+        *reinterpret_cast<u32x2*>(Kt + (((2 * kb + x / NI) * 2 + (w >> 1)) * NI + x % NI) * kFrag + lane * 8 + 4 * (w & 1)) = r;
       }
     }
+    const int dv = left > 0 ? a.Dv - col0 - 8 * g : 0;
 #pragma unroll
-    for (int x = 0; x < NW; ++x)
+    for (int b = 0; b < VB; ++b) {
+      const Terms<NI> v = terms_of<T>(vr[b], dv - 32 * b);
+      f32x4 z[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int cc = vc + 4 * x + i;
-        Vf[((cc >> 4) * 4 + w) * 256 + (16 * ((vt & 15) >> 2) + (cc & 15)) * 4 + (vt & 3)] =
-            c * C + vt < rows.n && col0 + cc < a.Dv ? vr[x][i] : (T)0.f;
+      for (int x = 0; x < 2; ++x) {
+        z[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = NI - 1; j >= 0; --j) z[x] = mfma(v.t[j], vsel[x], z[x]);
       }
-    for (int f = w; f < 4 * KB; f += 4) store_terms<NI>(Kt + f * NI * kFrag, lane, transposed<KB, NI>(Kf, f, lane));
-    Terms<NI> q[KB];
+      settle(z);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) q[kb] = row_terms(qr[kb], kb, c);
-    if (c + 1 < nch) fetch(c + 1);
+      for (int x = 0; x < 2; ++x)
+        if (2 * b + x < NW) *reinterpret_cast<f32x4*>(Vf + ((2 * b + x) * 4 + w) * 256 + lane * 4) = z[x];
+    }
+    Terms<NI> q[KB];
+    const int dk = left > 0 ? a.Dk - 8 * g : 0;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) q[kb] = terms_of<T>(qr[kb], dk - 32 * kb);
+    left -= C;
+    if (c + 1 < nch) fetch();
     if (c) write_out(c - 1);
     // P
     const float Gt = vec[V_G * C + t], Gl = vec[V_GLOW * C + t];
+    {
+      f32x4 y[4];
 #pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2) {
-      if (kb2 > w / 2) continue;
-      f32x4 y[2];
+      for (int jt = 0; jt < 4; ++jt) y[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int jt = 2 * kb2 + x;
-        y[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (jt <= w) {
+      for (int kb = 0; kb < KB; ++kb) {
+        Terms<NI> k[4];
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) y[x] = product<2>(load_terms<NI>(Kf + (jt * KB + kb) * NI * kFrag, lane), q[kb], y[x]);
-          settle(y[x]);
-          const f32x4 G = *reinterpret_cast<const f32x4*>(vec + V_G * C + 16 * jt + 4 * g);
-          const f32x4 L = *reinterpret_cast<const f32x4*>(vec + V_GLOW * C + 16 * jt + 4 * g);
+        for (int jt = 0; jt < 4; ++jt) k[jt] = load_terms<NI>(Kf + (jt * KB + kb) * NI * kFrag, lane);
+        products<2>(k, q[kb], y);
+      }
+      settle(y);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * jt + 4 * g + r;
-            y[x][r] = j <= t ? a.scale * expf((Gt - G[r]) + (Gl - L[r])) * y[x][r] : 0.f;
-          }
+      for (int jt = 0; jt < 4; ++jt) {
+        const f32x4 G = *reinterpret_cast<const f32x4*>(vec + V_G * C + 16 * jt + 4 * g);
+        const f32x4 L = *reinterpret_cast<const f32x4*>(vec + V_GLOW * C + 16 * jt + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float f = a.scale * exp2_fast((Gt - G[r]) + (Gl - L[r]));
+          y[jt][r] = 16 * jt + 4 * g + r <= t ? f * y[jt][r] : 0.f;
         }
       }
-      p[kb2] = split<NO>(y[0], y[1]);
+      p[0] = split<NO>(y[0], y[1]);
+      p[1] = split<NO>(y[2], y[3]);
     }
     lds_barrier();
     const float since = a.scale * vec[V_SINCE * C + t];
 #pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      O[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (col0 + 16 * x >= a.Dv) continue;
+    for (int x = 0; x < NW; ++x) O[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) O[x] = product<ORD>(load_terms<NO>(Sf + (x * KB + kb) * NO * kFrag, lane), q[kb], O[x]);
-      settle(O[x]);
-      O[x] *= since;
+    for (int kb = 0; kb < KB; ++kb) {
+      Terms<NO> y[NW];
+#pragma unroll
+      for (int x = 0; x < NW; ++x) y[x] = load_terms<NO>(Sf + (x * KB + kb) * NO * kFrag, lane);
+      products<ORD>(y, q[kb], O);
     }
+    settle(O);
+#pragma unroll
+    for (int x = 0; x < NW; ++x) O[x] *= since;
     if (c + 1 < nch) put_keys(c + 1);
     lds_barrier();
   }
@@ -663,7 +722,7 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
   for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int d = 16 * dt + 4 * g + i;
+      const int d = channel(dt, 4 * g + i);
       S[dt][i] = a.d_final && in && d < a.Dk ? a.d_final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
     }
   for (int64_t c = nch - 1; c >= 0; --c) {
@@ -674,7 +733,7 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
     for (int dt = 0; dt < 2 * KB; ++dt) *reinterpret_cast<f32x4*>(a.dstates + (cg * 2 * KB + dt) * 256 + lane * 4) = S[dt];
     constexpr int kAll = 4 * KB * NI * kFrag;
     const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
-    const __bf16* tri = tri_tiles(a, tile, h);
+    const __bf16* tri = tri_tiles<true>(a, tile, h);
     const float* vec = vec_of(a, tile, h);
     f32x4 dO[4];
 #pragma unroll
@@ -747,30 +806,28 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
     for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int d = 16 * dt + 4 * g + i;
+        const int d = channel(dt, 4 * g + i);
         if (in && d < a.Dk) a.d_init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
       }
   }
 }
 
-// One lane's eight values of a row: inner indices k0 + 4g + i and k0 + 16 + 4g + i, zero from
-// index `width` on.
+// One lane's eight values of a row, channels k0 + 8g.., of `width`.
 template <typename T>
 __device__ __forceinline__ void load8(const T* base, int64_t at, int k0, int g, int width, float (&x)[8]) {
-  const int d = k0 + 4 * g;
-  const f32x4 lo = load4(base, at + d, width - d), hi = load4(base, at + d + 16, width - d - 16);
+  const int d = k0 + 8 * g;
+  const Raw8<T> y = fetch8(base, at + d, width - d);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
+  for (int i = 0; i < 8; ++i) x[i] = width - d > 0 ? (float)y[i] : 0.f;
 }
 
-// Row r, columns c0 + 4g.. and c0 + 16 + 4g.. of a matrix that chain() or chain_back() kept as it
-// lay in registers, `tiles` tiles of 16 rows for each of the 16-column groups.
+// Row r, columns c0 + 8g.. of a matrix that chain() or chain_back() kept as it lay in
+// registers, `tiles` tiles of 16 rows for each of the 16-column groups.
 __device__ __forceinline__ void load_kept(const float* x, int tiles, int r, int c0, int g, int groups, float (&y)[8]) {
+  const int cg = c0 / 16 + (g >> 1);
+  const float* p = x + ((cg < groups ? cg : 0) * tiles + r / 16) * 256 + (16 * ((r & 15) / 4) + 8 * (g & 1)) * 4 + (r & 3);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int cg = c0 / 16 + (i >> 2);
-    y[i] = cg < groups ? x[(cg * tiles + r / 16) * 256 + (16 * ((r & 15) / 4) + 4 * g + (i & 3)) * 4 + (r & 3)] : 0.f;
-  }
+  for (int i = 0; i < 8; ++i) y[i] = cg < groups ? p[4 * i] : 0.f;
 }
 
 // Grid (tiles, Hk), four wavefronts; wavefront w has tokens 16w..16w+15, lane m the token
@@ -823,7 +880,7 @@ __global__ __launch_bounds__(256) void grads(Args a) {
       const Terms<NX> r = split<NX>(xr), u = split<NX>(xu);
 #pragma unroll
       for (int dt = 0; dt < 2 * KB; ++dt) {
-        const int d = 16 * dt + m;
+        const int d = 16 * dt + m;  // as kept
         float xs[8], xd[8];
         load_kept(St, 2 * KB, d, c0, g, a.groups, xs);
         load_kept(dSt, 2 * KB, d, c0, g, a.groups, xd);
@@ -869,7 +926,7 @@ __global__ __launch_bounds__(256) void grads(Args a) {
       hq[dt] *= a.scale * since;
       rho[dt] *= -since;
       kw[dt] *= left;
-      const f32x4 k = load4(kbase, t * a.kn + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0);
+      const f32x4 k = load4(kbase, t * a.kn + channel(dt, 4 * g), t < n ? a.Dk - channel(dt, 4 * g) : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) kend = fmaf(k[i], kw[dt][i], kend);
     }
@@ -882,7 +939,7 @@ __global__ __launch_bounds__(256) void grads(Args a) {
       for (int i = 0; i < 4; ++i) {
         const int y = 16 * x + 4 * g + i;
         const float d = (Gt - Gy[i]) + (Gl - Ly[i]);
-        const float fi = y <= t ? expf(d) : 0.f, fj = y >= t ? expf(-d) : 0.f;
+        const float fi = exp2_fast(d), fj = exp2_fast(-d);
         E1[x][i] = y <= t ? a.scale * fi * E1[x][i] : 0.f;
         E2[x][i] = y < t ? -fi * E2[x][i] : 0.f;
         F1[x][i] = y >= t ? a.scale * fj * F1[x][i] : 0.f;
@@ -912,8 +969,8 @@ __global__ __launch_bounds__(256) void grads(Args a) {
     }
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      const f32x4 k = load4(kbase, t * a.kn + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0);
-      const f32x4 q = load4(qbase, t * a.qn + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0);
+      const f32x4 k = load4(kbase, t * a.kn + channel(dt, 4 * g), t < n ? a.Dk - channel(dt, 4 * g) : 0);
+      const f32x4 q = load4(qbase, t * a.qn + channel(dt, 4 * g), t < n ? a.Dk - channel(dt, 4 * g) : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         qq = fmaf(q[i], hq[dt][i], qq);
@@ -953,9 +1010,10 @@ __global__ __launch_bounds__(256) void grads(Args a) {
     T* dkrow = (T*)a.dk + bt * a.dkb + hk * a.dkh + (row0 + t) * a.dkn;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      if (16 * dt + 4 * g >= a.Dk) continue;
-      store4(dqrow + 16 * dt + 4 * g, dq[dt]);
-      store4(dkrow + 16 * dt + 4 * g, dk[dt]);
+      const int d = channel(dt, 4 * g);
+      if (d >= a.Dk) continue;
+      store4(dqrow + d, dq[dt]);
+      store4(dkrow + d, dk[dt]);
     }
   }
 }
@@ -1075,13 +1133,13 @@ int64_t tiles_of(const kdelta_problem* p) {
 int input_terms(int dtype) { return dtype == KDECAY_BF16 ? 1 : dtype == KDECAY_F16 ? 2 : 3; }
 
 struct Sizes {  // bytes
-  size_t inv, keys, tris, vecs, dstates, drs;
+  size_t inv, keys, tris, vecs, dstates, drs;  // inv: the forward's T
 };
 
 Sizes sizes_of(const kdelta_problem* p) {
   const size_t tiles = tiles_of(p), KB = (p->Dk + 31) / 32, NI = input_terms(p->dtype), groups = (p->Dv + 15) / 16;
   Sizes s;
-  s.inv = up256(tiles * p->H * kTri * kFrag * 4);
+  s.inv = up256(tiles * p->H * kTri * NX * kFrag * 2);
   s.keys = up256(tiles * p->Hk * 3 * 4 * KB * NI * kFrag * 2);
   s.tris = up256(tiles * p->H * kTri * 2 * NX * kFrag * 2);
   s.vecs = up256(tiles * p->H * V_COUNT * C * 4);
@@ -1106,8 +1164,8 @@ int check(const kdelta_problem* p) {
   if (!p->cu_seqlens && p->sequences != p->B) return fail(KDECAY_EINVAL, "sequences must be B without cu_seqlens");
   if (p->sequences > 0x7fffffff || tiles_of(p) > 0x7fffffff) return fail(KDECAY_ESHAPE, "too many sequences or rows");
   if (p->B && p->N && (!p->q || !p->k || !p->v || !p->g || !p->beta)) return fail(KDECAY_EINVAL, "null pointer argument");
-  if (p->Dk % 4 || p->Dv % 4)
-    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not multiples of 4", (long long)p->Dk, (long long)p->Dv);
+  if (p->Dk % 8 || p->Dv % 8)
+    return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not multiples of 8", (long long)p->Dk, (long long)p->Dv);
   if (!p->B || !p->N) return 0;
   if (const int rc = check_rows(p->q, p->q_strides, p->dtype, "q")) return rc;
   if (const int rc = check_rows(p->k, p->k_strides, p->dtype, "k")) return rc;
@@ -1130,7 +1188,7 @@ Args args_of(const kdelta_problem* p, void* workspace, bool backward) {
   char* w = (char*)workspace;
   a.vecs = (float*)w, w += s.vecs;
   if (!backward) {
-    a.inv = (float*)w;
+    a.tris = (__bf16*)w;
   } else {
     a.keys = (__bf16*)w, w += s.keys;
     a.tris = (__bf16*)w, w += s.tris;

@@ -81,6 +81,19 @@ __device__ __forceinline__ f32x4 product(const Terms<NA>& a, const Terms<NB>& b,
   return acc;
 }
 
+// The same for M accumulators with one B each: neighbouring instructions are independent of each
+// other (one that adds to the result of the one before it waits for it).
+template <int ORDER, int M, int NA, int NB>
+__device__ __forceinline__ void products(const Terms<NA> (&a)[M], const Terms<NB>& b, f32x4* acc) {
+#pragma unroll
+  for (int s = ORDER; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (s - i >= 0 && s - i < NB)
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[m] = mfma(a[m].t[i], b.t[s - i >= 0 && s - i < NB ? s - i : 0], acc[m]);
+}
+
 // Terms that an input of type T has, exactly.
 template <typename T>
 inline constexpr int kInputTerms = 3;
@@ -89,17 +102,25 @@ inline constexpr int kInputTerms<__bf16> = 1;
 template <>
 inline constexpr int kInputTerms<_Float16> = 2;
 
-// Rows are whole fours of elements, aligned to four (the hosts' checks and copies see to it),
-// so four elements are all there or none of them is: n, the elements left, is 0 or
-// less, or 4 or more.
+// Rows are whole eights of elements, aligned to 16 bytes (the hosts' checks and copies see to it),
+// so four or eight elements are all there or none of them is: n, the elements left, is 0 or less,
+// or 4 (8) or more.
 template <typename T>
 using Raw4 = T __attribute__((ext_vector_type(4)));
+
+template <typename T>
+using Raw8 = T __attribute__((ext_vector_type(8)));
 
 // Loads that are to stay in flight: no branch that depends on the lane, and no conversion,
 // until the values are used.  base itself is read where there is nothing to read.
 template <typename T>
 __device__ __forceinline__ Raw4<T> fetch4(const T* base, int64_t at, int n) {
   return *reinterpret_cast<const Raw4<T>*>(base + (n > 0 ? at : 0));
+}
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> fetch8(const T* base, int64_t at, int n) {
+  return *reinterpret_cast<const Raw8<T>*>(base + (n > 0 ? at : 0));
 }
 
 template <typename T>
@@ -220,11 +241,12 @@ __device__ __forceinline__ void zero_outside(const int32_t* cu, int64_t sequence
       for (int d = thread; d < width; d += threads) x[r * row_stride + d] = (T)0.f;
 }
 
-// The hosts' check of one tensor of rows: channels adjacent, every row aligned to four elements.
+// The hosts' check of one tensor of rows: channels adjacent, every row aligned to 16 bytes.
 inline int check_rows(const void* p, const int64_t* strides, int dtype, const char* name) {
   if (strides[3] != 1) return fail(KDECAY_ELAYOUT, "%s: channel (d) stride must be 1", name);
-  if (((uintptr_t)p & (dtype == KDECAY_F32 ? 15u : 7u)) || strides[0] % 4 || strides[1] % 4 || strides[2] % 4)
-    return fail(KDECAY_ELAYOUT, "%s: base and strides must be multiples of four elements", name);
+  const int n = dtype == KDECAY_F32 ? 4 : 8;
+  if (((uintptr_t)p & 15u) || strides[0] % n || strides[1] % n || strides[2] % n)
+    return fail(KDECAY_ELAYOUT, "%s: base and strides must be multiples of 16 bytes", name);
   return 0;
 }
 

@@ -60,11 +60,11 @@ void check_float(const Tensor& t, const Tensor& q, const char* name) {
 Tensor as_float(const Tensor& t) { return t.to(at::kFloat).resolve_neg(); }
 
 // Whether the kernels read (and write) `t` as it lies: channels adjacent, every row aligned to
-// four elements.  For head dims that are multiples of 4.
+// 16 bytes.  For head dims that are multiples of 8.
 bool rows_ok(const Tensor& t) {
-  if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % (4 * t.element_size()) || t.stride(3) != 1) return false;
+  if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 || t.stride(3) != 1) return false;
   for (int64_t k = 0; k < 3; ++k)
-    if (t.size(k) > 1 && t.stride(k) % 4) return false;
+    if (t.size(k) > 1 && t.stride(k) * t.element_size() % 16) return false;
   return true;
 }
 
@@ -82,12 +82,12 @@ Tensor new_like(const Tensor& like) {
   return r;
 }
 
-// Channels (of dimension `dim`) padded with zeros to a multiple of 4.
-Tensor pad4(const Tensor& t, int64_t dim) {
+// Channels (of dimension `dim`) padded with zeros to a multiple of 8.
+Tensor pad8(const Tensor& t, int64_t dim) {
   const int64_t n = t.size(dim);
-  if (n % 4 == 0) return t;
+  if (n % 8 == 0) return t;
   std::vector<int64_t> pad(2 * (t.dim() - dim), 0);
-  pad.back() = 4 - n % 4;
+  pad.back() = 8 - n % 8;
   return at::constant_pad_nd(t, pad, 0);
 }
 
@@ -238,9 +238,9 @@ py::object delta_scan(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   require_hip(q_in, "q");
   cu = as_cu(cu);
   const double scale = scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(Dk));
-  Tensor q = as_rows(pad4(q_in, 3)), k = as_rows(pad4(k_in, 3)), v = as_rows(pad4(v_in, 3));
+  Tensor q = as_rows(pad8(q_in, 3)), k = as_rows(pad8(k_in, 3)), v = as_rows(pad8(v_in, 3));
   Tensor g = as_float(g_in), beta = as_float(beta_in);
-  if (init.defined()) init = pad4(pad4(as_float(init), 3), 2).contiguous();
+  if (init.defined()) init = pad8(pad8(as_float(init), 3), 2).contiguous();
   Tensor o, final;
   {
     py::gil_scoped_release nogil;
@@ -254,8 +254,8 @@ py::object delta_scan(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
       const Scanned r = delta_forward(problem(q, k, v, g, beta, cu, init, scale), v, want_final, false);
       o = r.o, final = r.final;
     }
-    if (Dv % 4) o = at::empty_like(v_in).copy_(o.narrow(3, 0, Dv));
-    if (want_final && (Dk % 4 || Dv % 4)) final = final.narrow(2, 0, Dk).narrow(3, 0, Dv).contiguous();
+    if (Dv % 8) o = at::empty_like(v_in).copy_(o.narrow(3, 0, Dv));
+    if (want_final && (Dk % 8 || Dv % 8)) final = final.narrow(2, 0, Dk).narrow(3, 0, Dv).contiguous();
   }
   return want_final ? py::object(py::make_tuple(o, final)) : py::cast(o);
 }
@@ -361,7 +361,7 @@ Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, std
   TORCH_CHECK(!grad_wanted({&q_in, &k_in, &v_in}),
               "kilat_amd: causal_attention has no backward; call it under torch.no_grad()");
   at::AutoDispatchBelowADInplaceOrView below;  // new buffers only: nothing to record
-  const Tensor q = as_rows(pad4(q_in, 3)), k = as_rows(pad4(k_in, 3)), v = as_rows(pad4(v_in, 3)), cu = as_cu(cu_any);
+  const Tensor q = as_rows(pad8(q_in, 3)), k = as_rows(pad8(k_in, 3)), v = as_rows(pad8(v_in, 3)), cu = as_cu(cu_any);
   const c10::DeviceGuard guard(q.device());
   // Laid out like q: rows of all heads together where q's are.
   const bool tokens = H > 1 && N > 1 && q_in.stride(1) < q_in.stride(2);
@@ -378,7 +378,7 @@ Tensor attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, std
   p.scale = static_cast<float>(scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(Dk)));
   p.dtype = code_of(q, "q");
   check_rc(kattn_fwd(&p, o.data_ptr(), strides(o).data(), stream_of(q)), "kattn_fwd");
-  if (Dv % 4) return empty(Dv).copy_(o.narrow(3, 0, Dv));
+  if (Dv % 8) return empty(Dv).copy_(o.narrow(3, 0, Dv));
   return o;
 }
 
