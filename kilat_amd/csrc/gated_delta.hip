@@ -36,6 +36,7 @@ constexpr int kOutOrder = sizeof(T) == 4 ? 2 : 1;
 
 // Per token of a chunk, floats: b e^G, b, e^G, e^(G_64 - G), and G log2(e) as the sum of two.
 enum Vec { V_BG, V_BETA, V_SINCE, V_LEFT, V_G, V_GLOW, V_COUNT };
+constexpr int V_CHAIN = 4;  // what chain() reads of them
 
 struct Args {
   const void *q, *k, *v;
@@ -48,7 +49,7 @@ struct Args {
   float scale;
   // scratch, by tile and head
   __bf16* keys;    // backward: [tiles][Hk][3][4 KB][NI][kFrag]: K, its transpose, Q's transpose
-  __bf16* tris;    // [tiles][H][kTri * NX][kFrag]: T (backward: [kTri * 2 * NX], T's transpose and P's)
+  __bf16* tris;    // [tiles][H][kTri * (NX + kOutTerms)][kFrag]: T and P (backward: [kTri * 2 * NX], transposed)
   float* vecs;     // [tiles][H][V_COUNT][C]
   float* states;   // saved: [tiles][H][16-column groups][2 KB][64][4], S at the chunk's start as it lies in registers
   float* us;       // saved: [tiles][H][16-column groups][4][64][4]: u
@@ -77,9 +78,11 @@ template <int KB, int NI>
 __device__ __forceinline__ __bf16* key_tiles(const Args& a, int64_t tile, int hk) {
   return a.keys + ((tile * a.Hk + hk) * 3) * (int64_t)(4 * KB * NI * kFrag);
 }
-template <bool BWD>
+template <typename T, bool BWD>
+constexpr int kTriSize = kTri * (NX + (BWD ? NX : kOutTerms<T>)) * kFrag;
+template <typename T, bool BWD>
 __device__ __forceinline__ __bf16* tri_tiles(const Args& a, int64_t tile, int h) {
-  return a.tris + (tile * a.H + h) * (int64_t)(kTri * (BWD ? 2 : 1) * NX * kFrag);
+  return a.tris + (tile * a.H + h) * (int64_t)kTriSize<T, BWD>;
 }
 __device__ __forceinline__ float* vec_of(const Args& a, int64_t tile, int h) {
   return a.vecs + (tile * a.H + h) * (int64_t)(V_COUNT * C);
@@ -162,7 +165,7 @@ __device__ __forceinline__ float fade(double x) {
 // prep: T of one chunk and value head (BWD: what the backward's products take)
 // --------------------------------------------------------------------------
 // Grid (tiles, H), four wavefronts; wavefront w has tokens 16w..16w+15 of the chunk.
-// Operand tiles of terms, forward: T.  BWD: T and P transposed, K, K transposed and Q transposed.
+// Operand tiles of terms, forward: T and P.  BWD: T and P transposed, K, K transposed and Q transposed.
 //
 // log decays are added up in 64 bits: the sums over a chunk can be far larger than
 // the differences that count.  One below -128 is taken as -128: e^-128 is 0 in 32 bits,
@@ -191,12 +194,12 @@ __global__ __launch_bounds__(256) void prep(Args a) {
   const int t = 16 * w + m;
   const T* kbase = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + row0 * a.kn;
   const T* qbase = (const T*)a.q + at.rows.batch * a.qb + hk * a.qh + row0 * a.qn;
-  Raw8<T> kr[KB], qr[BWD ? KB : 1];
+  Raw8<T> kr[KB], qr[KB];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     const int d = 32 * kb + 8 * g, left = t < n ? a.Dk - d : 0;
     kr[kb] = fetch8(kbase, t * a.kn + d, left);
-    if (BWD) qr[BWD ? kb : 0] = fetch8(qbase, t * a.qn + d, left);
+    qr[kb] = fetch8(qbase, t * a.qn + d, left);
   }
   if (w == 0) {
     const bool in = lane < n;
@@ -262,27 +265,32 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       As[i * LD + j] = j < i ? bs[i] * fade(Gs[i] - Gs[j]) * acc[x] : 0.f;
     }
   }
-  if constexpr (BWD) {  // P transposed: rows j of this wavefront
-    __bf16* tri = tri_tiles<true>(a, tile, h);
+  {  // P: rows i of this wavefront (BWD: transposed, rows j)
+    __bf16* tri = tri_tiles<T, BWD>(a, tile, h) + kTri * NX * kFrag;
+    constexpr int NO = BWD ? NX : kOutTerms<T>;
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
-      if (kb2 < w / 2) continue;
-      f32x4 p[2];
+      if (BWD ? kb2 < w / 2 : kb2 > w / 2) continue;
+      f32x4 p[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int it = 2 * kb2 + x;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int kb = 0; kb < KB; ++kb) {
+        Terms<NI> y[2];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-          acc = product<2>(load_terms<NI>(kq[1] + (it * KB + kb) * NI * kFrag, lane), kt[kb], acc);
-        settle(acc);
+        for (int x = 0; x < 2; ++x) y[x] = load_terms<NI>(kq[BWD ? 1 : 0] + ((2 * kb2 + x) * KB + kb) * NI * kFrag, lane);
+        if constexpr (BWD)
+          products<2>(y, kt[kb], p);
+        else
+          products<2>(y, terms_of<T>(qr[kb], t < n ? a.Dk - 32 * kb - 8 * g : 0), p);
+      }
+      settle(p);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int j = 16 * w + m, i = 16 * it + 4 * g + r;
-          p[x][r] = j <= i ? a.scale * fade(Gs[i] - Gs[j]) * acc[r] : 0.f;
+          const int other = 32 * kb2 + 16 * x + 4 * g + r, i = BWD ? other : t, j = BWD ? t : other;
+          p[x][r] = j <= i ? a.scale * fade(Gs[i] - Gs[j]) * p[x][r] : 0.f;
         }
-      }
-      store_terms<NX>(tri + (kTri + tri_upper(w, kb2)) * NX * kFrag, lane, split<NX>(p[0], p[1]));
+      store_terms<NO>(tri + (BWD ? tri_upper(w, kb2) : tri_lower(w, kb2)) * NO * kFrag, lane, split<NO>(p[0], p[1]));
     }
   }
   __syncthreads();
@@ -342,7 +350,7 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       x[i >> 2][i & 3] = BWD ? Ts[o * LD + t] : Ts[t * LD + o];
     }
     const int f = BWD ? tri_upper(w, kb2) : tri_lower(w, kb2);
-    store_terms<NX>(tri_tiles<BWD>(a, tile, h) + f * NX * kFrag, lane, split<NX>(x[0], x[1]));
+    store_terms<NX>(tri_tiles<T, BWD>(a, tile, h) + f * NX * kFrag, lane, split<NX>(x[0], x[1]));
   }
 }
 
@@ -399,20 +407,23 @@ __device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, 
 // A workgroup has 16 NW columns of one head's state: NW wavefronts that keep 16 each
 // (in registers, 32 bits), and four that feed them and write o.  What one chunk
 // costs is the chain S -> K S -> R -> U -> S, so everything else is taken off it:
-// the feeders fetch the next chunk's rows, lay K and its transpose out as operand
-// tiles in LDS, split T, and compute P and o (from S and U, which the chain leaves in
-// LDS as terms).  Two barriers per chunk, so that one buffer each is enough:
-//   first part   chain: splits S, K S          feeders: T, V and K' of this chunk to LDS,
-//                                              P of this chunk, o of the one before
-//   second part  chain: R, U, S                feeders: q S of this chunk, K of the next to LDS
+// the feeders fetch the next chunk's rows, lay K and its transpose, T and V out in LDS as
+// the chain reads them, and compute o from S and U, which the chain leaves in LDS as terms.
+// Two barriers per chunk, so that one buffer each is enough (two of U where LDS has room:
+// then the products of P and U are off the first part, the shorter one of the chain's):
+//   first part   chain: splits S, K S     feeders: T, V and K' of this chunk to LDS
+//   second part  chain: R, U, S           feeders: fetch the next chunk, P U of the one before,
+//                                         q S of this one, K of the next to LDS
 template <typename T, int KB, int NW, bool SAVE>
 __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>, ORD = kOutOrder<T>;
   __shared__ __bf16 Kf[4 * KB * NI * kFrag], Kt[4 * KB * NI * kFrag], Tf[kTri * NX * kFrag];
   __shared__ float Vf[NW * 4 * 256];
-  __shared__ __bf16 Sf[NW * KB * NO * kFrag], Uf[NW * 2 * NO * kFrag];
-  __shared__ float vecs[2][V_COUNT * C];
-  __shared__ int by_token[NW];
+  constexpr int kLds = (8 * KB * NI + kTri * NX + NW * KB * NO) * 1024 + NW * 4096 + 2 * V_CHAIN * C * 4 + 64;
+  constexpr int UB = kLds + 2 * NW * 2 * NO * 1024 <= 160 * 1024 ? 2 : 1;  // buffers of U's terms
+  __shared__ __bf16 Sf[NW * KB * NO * kFrag], Uf[UB][NW * 2 * NO * kFrag];
+  __shared__ float vecs[2][V_CHAIN * C];
+  __shared__ int by_token[2][NW];
   const int64_t seq = blockIdx.x;
   const int h = blockIdx.y, hk = h / a.group;
   const int wave = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -491,7 +502,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) odd += U[mt][i];
         const bool slow = __any(!(fabsf(odd) <= 3.402823466e38f));  // something is not finite
-        if (lane == 0) by_token[wave] = slow;
+        if (lane == 0) by_token[c & 1][wave] = slow;
         if (slow) {
           chunk_by_token<T, KB, SAVE>(a, rows, rows.first + c * C, rows.n - c * C < C ? (int)(rows.n - c * C) : C, h, col,
                                       tile, S);
@@ -503,7 +514,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
             const Terms<NO> u = split<NO>(U[2 * kb], U[2 * kb + 1]);
-            store_terms<NO>(Uf + (wave * 2 + kb) * NO * kFrag, lane, u);
+            store_terms<NO>(Uf[c & (UB - 1)] + (wave * 2 + kb) * NO * kFrag, lane, u);
           }
           const float whole = vec[V_SINCE * C + C - 1];
 #pragma unroll
@@ -544,10 +555,12 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   constexpr int VB = (NW + 1) / 2;             // 32-column blocks of V
   constexpr int TP = (kTri * NX + 3) / 4;      // planes of T per feeder: w, w + 4, ...
   const T *kp = kbase + t * a.kn + 8 * g, *qp = qbase + t * a.qn + 8 * g, *vp = vbase + t * a.vn + col0 + 8 * g;
-  const __bf16* ip = tri_tiles<false>(a, tile0, h) + w * kFrag + lane * 8;
-  const float* ep = vec_of(a, tile0, h) + (ft % (V_COUNT * C / 4)) * 4;
+  const __bf16* ip = tri_tiles<T, false>(a, tile0, h) + w * kFrag + lane * 8;
+  const __bf16* pp = tri_tiles<T, false>(a, tile0, h) + (kTri * NX + tri_lower(w, 0) * NO) * kFrag + lane * 8;
+  const float* ep = vec_of(a, tile0, h) + (ft % (V_CHAIN * C / 4)) * 4;
   Raw8<T> kr[KB], qr[KB], vr[VB];
   bf16x8 tr[TP];
+  Terms<NO> pr[2] = {};
   f32x4 er;
   int left = rows.n < t ? 0 : rows.n - t < 0x7fffffff ? (int)(rows.n - t) : 0x7fffffff;  // rows from this lane's on
   const auto fetch = [&]() {  // the next chunk's
@@ -562,9 +575,11 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
 #pragma unroll
     for (int x = 0; x < TP; ++x)
       if (4 * x + 4 <= kTri * NX || w + 4 * x < kTri * NX) tr[x] = *reinterpret_cast<const bf16x8*>(ip + 4 * x * kFrag);
+    pr[0] = load_terms<NO>(pp, 0);
+    if (w >= 2) pr[1] = load_terms<NO>(pp + NO * kFrag, 0);
     er = *reinterpret_cast<const f32x4*>(ep);
     kp += C * a.kn, qp += C * a.qn, vp += C * a.vn;
-    ip += a.H * (int64_t)(kTri * NX * kFrag), ep += a.H * (int64_t)(V_COUNT * C);
+    ip += a.H * (int64_t)kTriSize<T, false>, pp += a.H * (int64_t)kTriSize<T, false>, ep += a.H * (int64_t)(V_COUNT * C);
   };
   Terms<NI> kt[KB];
   const auto put_keys = [&](int64_t c) {
@@ -574,7 +589,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
       kt[kb] = terms_of<T>(kr[kb], dk - 32 * kb);
       store_terms<NI>(Kf + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
     }
-    if (ft < V_COUNT * C / 4) *reinterpret_cast<f32x4*>(vecs[c & 1] + ft * 4) = er;
+    if (ft < V_CHAIN * C / 4) *reinterpret_cast<f32x4*>(vecs[c & 1] + ft * 4) = er;
   };
   // Columns of a 32-channel block of K in the order of a state's rows, and of V in its own.
   const bf16x8 ksel[2] = {selector(channel(0, m), g), selector(channel(1, m), g)};
@@ -584,7 +599,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   lds_barrier();
   Terms<NO> p[2];  // P of the last chunk: lane m = token i, inner indices j
   f32x4 O[NW];     // scale e^G S' q of it
-  const auto write_out = [&](int64_t c) {
+  const auto write_out = [&](int64_t c, const Terms<NO> (&p)[2], const f32x4 (&O)[NW]) {
     f32x4 y[NW];
 #pragma unroll
     for (int x = 0; x < NW; ++x) y[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -592,14 +607,14 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     for (int kb = 0; kb < 2; ++kb) {
       Terms<NO> u[NW];
 #pragma unroll
-      for (int x = 0; x < NW; ++x) u[x] = load_terms<NO>(Uf + (x * 2 + kb) * NO * kFrag, lane);
+      for (int x = 0; x < NW; ++x) u[x] = load_terms<NO>(Uf[c & (UB - 1)] + (x * 2 + kb) * NO * kFrag, lane);
       products<ORD>(u, p[kb], y);
     }
     settle(y);
     T* row = obase + (c * C + t) * a.on + col0 + 4 * g;
 #pragma unroll
     for (int x = 0; x < NW; ++x)
-      if (c * C + t < rows.n && col0 + 16 * x + 4 * g < a.Dv && !by_token[x]) store4(row + 16 * x, O[x] + y[x]);
+      if (c * C + t < rows.n && col0 + 16 * x + 4 * g < a.Dv && !by_token[c & 1][x]) store4(row + 16 * x, O[x] + y[x]);
   };
   for (int64_t c = 0; c < nch; ++c) {
     const float* vec = vecs[c & 1];
@@ -641,36 +656,12 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) q[kb] = terms_of<T>(qr[kb], dk - 32 * kb);
     left -= C;
-    if (c + 1 < nch) fetch();
-    if (c) write_out(c - 1);
-    // P
-    const float Gt = vec[V_G * C + t], Gl = vec[V_GLOW * C + t];
-    {
-      f32x4 y[4];
-#pragma unroll
-      for (int jt = 0; jt < 4; ++jt) y[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        Terms<NI> k[4];
-#pragma unroll
-        for (int jt = 0; jt < 4; ++jt) k[jt] = load_terms<NI>(Kf + (jt * KB + kb) * NI * kFrag, lane);
-        products<2>(k, q[kb], y);
-      }
-      settle(y);
-#pragma unroll
-      for (int jt = 0; jt < 4; ++jt) {
-        const f32x4 G = *reinterpret_cast<const f32x4*>(vec + V_G * C + 16 * jt + 4 * g);
-        const f32x4 L = *reinterpret_cast<const f32x4*>(vec + V_GLOW * C + 16 * jt + 4 * g);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float f = a.scale * exp2_fast((Gt - G[r]) + (Gl - L[r]));
-          y[jt][r] = 16 * jt + 4 * g + r <= t ? f * y[jt][r] : 0.f;
-        }
-      }
-      p[0] = split<NO>(y[0], y[1]);
-      p[1] = split<NO>(y[2], y[3]);
-    }
+    if (UB == 1 && c) write_out(c - 1, p, O);
+    const Terms<NO> p1[2] = {pr[0], pr[1]};
     lds_barrier();
+    if (c + 1 < nch) fetch();
+    if (UB == 2 && c) write_out(c - 1, p, O);
+    p[0] = p1[0], p[1] = p1[1];
     const float since = a.scale * vec[V_SINCE * C + t];
 #pragma unroll
     for (int x = 0; x < NW; ++x) O[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -687,7 +678,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     if (c + 1 < nch) put_keys(c + 1);
     lds_barrier();
   }
-  write_out(nch - 1);
+  write_out(nch - 1, p, O);
 }
 
 // --------------------------------------------------------------------------
@@ -733,7 +724,7 @@ __global__ __launch_bounds__(256) void chain_back(Args a) {
     for (int dt = 0; dt < 2 * KB; ++dt) *reinterpret_cast<f32x4*>(a.dstates + (cg * 2 * KB + dt) * 256 + lane * 4) = S[dt];
     constexpr int kAll = 4 * KB * NI * kFrag;
     const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
-    const __bf16* tri = tri_tiles<true>(a, tile, h);
+    const __bf16* tri = tri_tiles<T, true>(a, tile, h);
     const float* vec = vec_of(a, tile, h);
     f32x4 dO[4];
 #pragma unroll
@@ -1133,13 +1124,13 @@ int64_t tiles_of(const kdelta_problem* p) {
 int input_terms(int dtype) { return dtype == KDECAY_BF16 ? 1 : dtype == KDECAY_F16 ? 2 : 3; }
 
 struct Sizes {  // bytes
-  size_t inv, keys, tris, vecs, dstates, drs;  // inv: the forward's T
+  size_t inv, keys, tris, vecs, dstates, drs;  // inv: the forward's T and P
 };
 
 Sizes sizes_of(const kdelta_problem* p) {
   const size_t tiles = tiles_of(p), KB = (p->Dk + 31) / 32, NI = input_terms(p->dtype), groups = (p->Dv + 15) / 16;
   Sizes s;
-  s.inv = up256(tiles * p->H * kTri * NX * kFrag * 2);
+  s.inv = up256(tiles * p->H * kTri * (NX + (p->dtype == KDECAY_F32 ? 3 : 2)) * kFrag * 2);
   s.keys = up256(tiles * p->Hk * 3 * 4 * KB * NI * kFrag * 2);
   s.tris = up256(tiles * p->H * kTri * 2 * NX * kFrag * 2);
   s.vecs = up256(tiles * p->H * V_COUNT * C * 4);
