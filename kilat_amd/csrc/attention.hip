@@ -87,6 +87,11 @@ __device__ __forceinline__ f32x16 product32(const Operand<T>& a, const Operand<T
   return acc;
 }
 
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
 struct Args {
   const void *q, *k, *v;
   void* o;
@@ -107,6 +112,12 @@ __device__ __forceinline__ void load_row8(const T* base, int64_t at, int n, floa
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
+
+// float32: rows pass registers, where they are split into terms.
 // KS: steps of 16 channels of q and k; VT: tiles of 32 channels of v.
 template <typename T, int KS, int VT>
 __global__ __launch_bounds__(kThreads) void forward(Args a) {
@@ -228,7 +239,7 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
     top = fmaxf(top, __shfl_xor(top, 32));
     const float m1 = fmaxf(m, top), base = m1 == -INFINITY ? 0.f : m1;
     if (__any(m1 > m)) {
-      const float f = exp2f(m - base);
+      const float f = exp2_fast(m - base);
       l *= f;
 #pragma unroll
       for (int t = 0; t < VT; ++t) O[t] *= f;
@@ -239,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
       float p[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = exp2f(S[t][r] - base);
+        p[r] = exp2_fast(S[t][r] - base);
         l += p[r];
       }
 #pragma unroll
@@ -283,6 +294,256 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
     }
 }
 
+// --------------------------------------------------------------------------
+// 16-bit types
+// --------------------------------------------------------------------------
+// Keys and values go from global memory to LDS without passing registers, the next 64
+// rows while these are computed on (two buffers, one barrier per step), as rows of
+// 16-byte chunks; a row's chunks are permuted by an exclusive or with its number, so
+// that neither the 32 rows that a key operand reads nor the eight that a value
+// operand reads lie in the same banks.  Values are transposed by the LDS read.
+template <int CPR>
+__device__ __forceinline__ int swizzle(int row) {
+  return CPR == 16 ? row & 15 : (row >> 1) & 7;
+}
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes per lane from global memory to LDS, at `to` + 16 lane.  In assembly, because the compiler
+// takes the LDS that its own form of it writes for any LDS that is read later, and
+// waits for the next step's rows before it reads this one's; the loop waits itself.
+__device__ __forceinline__ void copy_to_lds(const void* from, const void* to) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LdsPtr)(void*)to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
+
+// One wavefront's share of a tile of 64 rows of CPR chunks: NL instructions of 64 chunks.
+template <typename T, int CPR>
+struct Stage {
+  static constexpr int NL = CPR / kWaves;
+  const T* p[NL];
+  int row[NL];
+  bool on[NL];  // the channels are the tensor's, not the tile's padding
+  __device__ __forceinline__ void init(const T* base, int64_t stride, int width, int w, int lane) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = (w * NL + i) * 64 + lane, chunk = c % CPR;
+      row[i] = c / CPR;
+      const int d = (chunk ^ swizzle<CPR>(row[i])) * 8;
+      on[i] = d < width;
+      p[i] = base + row[i] * stride + d;
+    }
+  }
+  // Rows k0.. of n, into `to`; rows behind the last are copies of it.
+  __device__ __forceinline__ void load(T* to, int64_t k0, int64_t n, int64_t stride, int w) {
+    if (k0 + BK <= n) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (on[i]) copy_to_lds(p[i], to + (w * NL + i) * 512);
+    } else {
+      const int last = (int)(n - 1 - k0);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int over = row[i] > last ? row[i] - last : 0;
+        if (on[i]) copy_to_lds(p[i] - over * stride, to + (w * NL + i) * 512);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) p[i] += BK * stride;
+  }
+};
+
+// The halves of a word that are infinite or NaN, as masks of 16 bits.
+template <typename T>
+__device__ __forceinline__ unsigned not_finite(unsigned x) {
+  constexpr unsigned top = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
+  return (((x & 0x7fff7fffu) + top) >> 15 & 0x00010001u) * 0xffffu;
+}
+
+template <typename T, int KS, int VT>
+__global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
+  typedef typename Vec8<T>::type V8;
+  constexpr int KC = 2 * KS, VC = 4 * VT;  // chunks of a row
+  __shared__ __align__(16) T kbuf[2][BK * KC * 8], vbuf[2][BK * VC * 8];
+  // Workgroups go to the eight XCDs in turn.  With a multiple of eight heads each XCD has heads of
+  // its own, so the keys that its workgroups read at the same time are the same; the tiles
+  // with the most keys go first.
+  const unsigned id = blockIdx.x, H = a.H, tiles = (unsigned)a.tiles;
+  const unsigned per = a.H % 8 ? H : H / 8, lane_of = a.H % 8 ? id : id / 8;
+  const unsigned order = lane_of / per;
+  const int h = (int)((a.H % 8 ? 0 : id % 8 * per) + lane_of % per);
+  int64_t tile = tiles - 1 - order;
+  if (!a.cu) {
+    const unsigned seqs = (unsigned)a.sequences, each = tiles / seqs;
+    tile = order % seqs * (int64_t)each + (each - 1 - order / seqs);
+  }
+  const int hk = h / a.group;
+  const int tid = threadIdx.x, w = wave_index(), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
+  zero_outside<BQ>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, tid, kThreads);
+  const TileOf at = tile_of<BQ>(a.cu, a.sequences, tile, a.N);
+  const int64_t q0 = at.index * BQ, n = at.rows.n;
+  if (n <= q0) return;
+  const T* kp = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + at.rows.first * a.kn;
+  const T* vp = (const T*)a.v + at.rows.batch * a.vb + hk * a.vh + at.rows.first * a.vn;
+  if (a.Dk < KS * 16 || a.Dv < VT * 32) {  // padding chunks are zero throughout
+    for (int i = tid; i < 2 * BK * KC; i += kThreads) reinterpret_cast<uint4*>(kbuf)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < 2 * BK * VC; i += kThreads) reinterpret_cast<uint4*>(vbuf)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  Stage<T, KC> sk;
+  Stage<T, VC> sv;
+  sk.init(kp, a.kn, a.Dk, w, lane);
+  sv.init(vp, a.vn, a.Dv, w, lane);
+  sk.load(kbuf[0], 0, n, a.kn, w);
+  sv.load(vbuf[0], 0, n, a.vn, w);
+  const int64_t row = q0 + 32 * w + n32;  // of the sequence
+  const bool live = row < n;
+  const bool flip = a.scale < 0.f;  // scores of -q and the scale's size
+  V8 q[KS];
+  {
+    const T* p = (const T*)a.q + at.rows.batch * a.qb + h * a.qh + at.rows.first * a.qn;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int left = live ? a.Dk - 16 * s - 8 * half : 0;
+      const Raw8<T> x = fetch8(p, row * a.qn + 16 * s + 8 * half, left);
+      uint4 y = __builtin_bit_cast(uint4, x);
+      const unsigned sign = flip ? 0x80008000u : 0u;
+      y = left > 0 ? make_uint4(y.x ^ sign, y.y ^ sign, y.z ^ sign, y.w ^ sign) : make_uint4(0, 0, 0, 0);
+      q[s] = __builtin_bit_cast(V8, y);
+    }
+  }
+  // Where this lane reads: key operands, row n32 of a tile of 32, chunk 2s + half; value operands, by
+  // 16 lanes, four keys (of half's four) of 16 channels.
+  const int kat = n32 * KC * 16, kx = half ^ swizzle<KC>(n32);
+  const int j = lane & 15, vrow = 4 * half + (j >> 2);
+  const int vat = vrow * VC * 16 + (j & 1) * 8, vx = (2 * ((lane >> 4) & 1) + ((j >> 1) & 1)) ^ swizzle<VC>(vrow);
+  f32x16 O[VT];
+#pragma unroll
+  for (int t = 0; t < VT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) O[t][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const float to2 = fabsf(a.scale) * 1.44269504088896340736f;  // scores in powers of 2
+  const int64_t last = q0 + BQ < n ? q0 + BQ : n;
+  const int steps = (int)((last + BK - 1) / BK), mine = (int)((q0 + 32 * w + 32 + BK - 1) / BK);  // of this wavefront's rows
+
+  const auto step = [&](int i, auto masked_of) {
+    constexpr bool masked = decltype(masked_of)::value;
+    const char* kl = reinterpret_cast<const char*>(kbuf[i & 1]);
+    const char* vl = reinterpret_cast<const char*>(vbuf[i & 1]);
+    const int seen = masked ? (int)(row - (int64_t)i * BK) : 0;  // the last key of the step that the row sees
+    f32x16 S[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        S[t] = mfma32(*reinterpret_cast<const V8*>(kl + t * 32 * KC * 16 + kat + ((kx ^ (2 * s)) << 4)), q[s], S[t]);
+    if (masked) settle(S);
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (masked) S[t][r] = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) <= seen ? S[t][r] : -INFINITY;
+        top = fmaxf(top, S[t][r]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 32)) * to2;
+    if (masked) top = seen < 0 ? -INFINITY : top;  // (to2 may be 0)
+    // The maximum that is subtracted may be up to 8 (in powers of 2) below the true one: sums stay
+    // far from 32 bits' end, and the rescaling of earlier sums is rare.
+    // (Row by row: what one row's scores are changes no digit of another's result.)
+    const bool raise = top > m + 8.f || (m == -INFINITY && top > m);
+    if (__any(raise)) {
+      const float m1 = raise ? top : m, f = !raise ? 1.f : m == -INFINITY ? 0.f : exp2_fast(m - m1);
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) O[t] *= f;
+      m = m1;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    unsigned bad = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        V8 p;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          float x = exp2_fast(fmaf(S[t][8 * s + r], to2, -base));
+          if (masked) x = 32 * t + 16 * s + 8 * (r >> 2) + 4 * half + (r & 3) <= seen ? x : 0.f;
+          l += x;
+          p[r] = (T)x;
+        }
+#pragma unroll
+        for (int vt = 0; vt < VT; ++vt) {
+          s16x4 y[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            y[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(vl + (32 * t + 16 * s + 8 * b) * VC * 16 + vat +
+                                                           ((vx ^ (4 * vt) ^ swizzle<VC>(8 * b)) << 4)));
+          uint4 z = make_uint4(__builtin_bit_cast(u32x2, y[0]).x, __builtin_bit_cast(u32x2, y[0]).y,
+                               __builtin_bit_cast(u32x2, y[1]).x, __builtin_bit_cast(u32x2, y[1]).y);
+          if (masked) {
+            const unsigned bx = not_finite<T>(z.x), by = not_finite<T>(z.y), bz = not_finite<T>(z.z), bw = not_finite<T>(z.w);
+            bad |= bx | by | bz | bw;
+            z = make_uint4(z.x & ~bx, z.y & ~by, z.z & ~bz, z.w & ~bw);
+          }
+          O[vt] = mfma32(__builtin_bit_cast(V8, z), p, O[vt]);
+        }
+      }
+    }
+    if (masked) {
+      settle(O);
+      if (__any(bad)) {
+        // Values that are not finite were taken as 0: they count for the rows from their own on only.
+        const int64_t k0 = (int64_t)i * BK;
+        for (int key = 0; key < BK; ++key)
+          if (key <= seen && k0 + key < n)
+#pragma unroll
+            for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int c = 32 * vt + 8 * (r >> 2) + 4 * half + (r & 3);
+                const float x = c < a.Dv ? (float)vp[(k0 + key) * a.vn + c] : 0.f;
+                if (!finite(x)) O[vt][r] += x;
+              }
+      }
+    }
+  };
+  for (int i = 0; i < steps; ++i) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wavefront's rows of the step are in LDS
+    __syncthreads();
+    if (i + 1 < steps) {
+      sk.load(kbuf[(i + 1) & 1], (int64_t)(i + 1) * BK, n, a.kn, w);
+      sv.load(vbuf[(i + 1) & 1], (int64_t)(i + 1) * BK, n, a.vn, w);
+    }
+    if (i >= mine) continue;  // every key is behind this wavefront's rows
+    if ((int64_t)(i + 1) * BK <= q0 + 32 * w)
+      step(i, Bool<false>());
+    else
+      step(i, Bool<true>());
+  }
+  settle(O);
+  l += __shfl_xor(l, 32);
+  if (!live) return;
+  T* p = (T*)a.o + at.rows.batch * a.ob + h * a.oh + (at.rows.first + row) * a.on;
+  const float il = 1.f / l;
+#pragma unroll
+  for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int c = 32 * vt + 2 * r + 4 * half;
+      const f32x4 x = {O[vt][r] * il, O[vt][r + 1] * il, O[vt][r + 2] * il, O[vt][r + 3] * il};
+      if (c < a.Dv) store4(p + c, x);
+    }
+}
+
 template <int BLOCK>
 int64_t tiles_of(const kattn_problem* p) {
   return p->cu_seqlens ? p->N / BLOCK + p->sequences : p->B * ((p->N + BLOCK - 1) / BLOCK);
@@ -303,7 +564,7 @@ int check(const kattn_problem* p, const void* o, const int64_t* o_strides) {
   if (p->cu_seqlens && (p->B != 1 || p->sequences < 1))
     return fail(KDECAY_ESHAPE, "cu_seqlens takes B=1 and at least one sequence");
   if (!p->cu_seqlens && p->sequences != p->B) return fail(KDECAY_EINVAL, "sequences must be B without cu_seqlens");
-  if (p->sequences > 0x7fffffff || tiles_of<32>(p) > 0x7fffffff)
+  if (p->sequences > 0x7fffffff || tiles_of<BQ>(p) * p->H > 0x7fffffff)
     return fail(KDECAY_ESHAPE, "too many sequences or rows");
   if (p->Dk % 8 || p->Dv % 8)
     return fail(KDECAY_ESHAPE, "head dims Dk=%lld, Dv=%lld are not multiples of 8", (long long)p->Dk, (long long)p->Dv);
@@ -336,16 +597,22 @@ extern "C" int kattn_fwd(const kattn_problem* p, void* o, const int64_t* o_strid
   a.scale = p->scale;
   const auto launch = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const dim3 grid((unsigned)a.tiles, a.H);
     const hipStream_t s = (hipStream_t)stream;
+    const auto with = [&](auto ks, auto vt) {
+      constexpr int KS = decltype(ks)::value, VT = decltype(vt)::value;
+      if constexpr (sizeof(T) == 2)
+        forward16<T, KS, VT><<<dim3((unsigned)(a.tiles * a.H)), kThreads, 0, s>>>(a);
+      else
+        forward<T, KS, VT><<<dim3((unsigned)a.tiles, a.H), kThreads, 0, s>>>(a);
+    };
     if (a.Dk <= 64 && a.Dv <= 64)
-      forward<T, 4, 2><<<grid, kThreads, 0, s>>>(a);
+      with(Int<4>(), Int<2>());
     else if (a.Dk <= 64)
-      forward<T, 4, 4><<<grid, kThreads, 0, s>>>(a);
+      with(Int<4>(), Int<4>());
     else if (a.Dv <= 64)
-      forward<T, 8, 2><<<grid, kThreads, 0, s>>>(a);
+      with(Int<8>(), Int<2>());
     else
-      forward<T, 8, 4><<<grid, kThreads, 0, s>>>(a);
+      with(Int<8>(), Int<4>());
     return hip_check("kattn_fwd launch");
   };
   if (p->dtype == KDECAY_BF16) return launch((__bf16*)nullptr);

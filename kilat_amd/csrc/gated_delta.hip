@@ -151,10 +151,6 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// 2^x, by the instruction: x is a difference of two sums of log decays, exact to 2^-24 of
-// itself, so what is at most 1 is off by 2^-24 x 2^x, less than its last digit.
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
 // e^x for a difference of sums of log decays (positive for a growing state only).
 __device__ __forceinline__ float fade(double x) {
   const float hi = (float)x, e = expf(hi);

@@ -163,6 +163,9 @@ __device__ __forceinline__ void settle(V (&x)[N]) {
 // lanes: branches on it are scalar, and barriers behind them are reached by whole wavefronts.
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
+// 2^x, by the instruction.
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // Sum over the four lane groups (lanes l, l^16, l^32, l^48).
 __device__ __forceinline__ float group_sum(float x) {
   x += __shfl_xor(x, 16);
@@ -205,7 +208,7 @@ template <int C>
 __device__ __forceinline__ TileOf tile_of(const int32_t* cu, int64_t sequences, int64_t tile, int64_t N) {
   int64_t s;
   if (!cu) {
-    s = tile / ((N + C - 1) / C);
+    s = (unsigned)tile / (unsigned)((N + C - 1) / C);  // (tiles are fewer than 2^31)
   } else {
     int64_t lo = 0, hi = sequences;  // the last s whose first tile is not behind `tile`
     while (hi - lo > 1) {
