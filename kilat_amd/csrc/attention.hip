@@ -307,17 +307,6 @@ __device__ __forceinline__ int swizzle(int row) {
   return CPR == 16 ? row & 15 : (row >> 1) & 7;
 }
 
-typedef __attribute__((address_space(3))) void* LdsPtr;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-// 16 bytes per lane from global memory to LDS, at `to` + 16 lane.  In assembly, because the compiler
-// takes the LDS that its own form of it writes for any LDS that is read later, and
-// waits for the next step's rows before it reads this one's; the loop waits itself.
-__device__ __forceinline__ void copy_to_lds(const void* from, const void* to) {
-  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LdsPtr)(void*)to);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
-}
-
 // One wavefront's share of a tile of 64 rows of CPR chunks: NL instructions of 64 chunks.
 template <typename T, int CPR>
 struct Stage {
@@ -481,14 +470,11 @@ __global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
         }
 #pragma unroll
         for (int vt = 0; vt < VT; ++vt) {
-          s16x4 y[2];
+          u32x2 y[2];
 #pragma unroll
           for (int b = 0; b < 2; ++b)
-            y[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(vl + (32 * t + 16 * s + 8 * b) * VC * 16 + vat +
-                                                           ((vx ^ (4 * vt) ^ swizzle<VC>(8 * b)) << 4)));
-          uint4 z = make_uint4(__builtin_bit_cast(u32x2, y[0]).x, __builtin_bit_cast(u32x2, y[0]).y,
-                               __builtin_bit_cast(u32x2, y[1]).x, __builtin_bit_cast(u32x2, y[1]).y);
+            y[b] = read_transposed(vl + (32 * t + 16 * s + 8 * b) * VC * 16 + vat + ((vx ^ (4 * vt) ^ swizzle<VC>(8 * b)) << 4));
+          uint4 z = make_uint4(y[0].x, y[0].y, y[1].x, y[1].y);
           if (masked) {
             const unsigned bx = not_finite<T>(z.x), by = not_finite<T>(z.y), bz = not_finite<T>(z.z), bw = not_finite<T>(z.w);
             bad |= bx | by | bz | bw;
@@ -517,7 +503,7 @@ __global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
     }
   };
   for (int i = 0; i < steps; ++i) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wavefront's rows of the step are in LDS
+    lds_copies_done();  // this wavefront's rows of the step are in LDS
     __syncthreads();
     if (i + 1 < steps) {
       sk.load(kbuf[(i + 1) & 1], (int64_t)(i + 1) * BK, n, a.kn, w);

@@ -45,14 +45,15 @@ struct Args {
   const float* init;
   int64_t qb, qh, qn, kb, kh, kn, vb, vh, vn, gb, gh, gn, bb, bh, bn;
   int64_t N, sequences, tiles;
-  int Hk, H, Dk, Dv, group, groups;  // value heads of a key head; 16-column groups of Dv
+  int Hk, H, Dk, Dv, group;  // group: value heads of a key head
+  int blocks, groups;        // blocks of 32 columns of v, and their groups of 16
   float scale;
   // scratch, by tile and head
-  __bf16* keys;    // backward: [tiles][Hk][3][4 KB][NI][kFrag]: K, its transpose, Q's transpose
-  __bf16* tris;    // [tiles][H][kTri * (NX + kOutTerms)][kFrag]: T and P (backward: [kTri * 2 * NX], transposed)
-  float* vecs;     // [tiles][H][V_COUNT][C]
-  float* states;   // saved: [tiles][H][16-column groups][2 KB][64][4], S at the chunk's start as it lies in registers
-  float* us;       // saved: [tiles][H][16-column groups][4][64][4]: u
+  __bf16* tris;     // [tiles][H][kTri * (NX + kOutTerms)][kFrag]: T and P (backward: [kTri * NX], T's transpose)
+  float* vecs;      // [tiles][H][V_COUNT][C]
+  // Kept for the backward, as planes of terms (see plane_at): S at the chunk's start and u, saved
+  __bf16* states;   // [tiles][H][blocks][NX][32][32 KB]
+  __bf16* us;       // [tiles][H][blocks][NX][32][C]
   void* o;
   int64_t ob, oh, on;
   float* final;
@@ -61,8 +62,10 @@ struct Args {
   int64_t dob, doh, don;
   const float* d_final;
   float* d_init;
-  float* dstates;  // [tiles][H][Dk][Dv], the gradient of the state at the chunk's end
-  float* drs;      // [tiles][H][C][Dv], the gradient of R
+  float* ys;        // [tiles][H][groups][4][64][4]: P' dO, as it lies in registers
+  float* zs;        // [tiles][H][groups][2 KB][64][4]: scale Q' (e^G dO)
+  __bf16* dstates;  // like states: the gradient of the state at the chunk's end
+  __bf16* drs;      // like us: the gradient of R
   void *dq, *dk, *dv;
   int64_t dqb, dqh, dqn, dkb, dkh, dkn, dvb, dvh, dvn;
   float *dg, *dbeta;
@@ -73,19 +76,72 @@ struct Args {
 // a state, are the channels 8g..8g+7: an operand of k's rows is loaded as they lie.
 __host__ __device__ constexpr int channel(int dt, int r) { return 32 * (dt >> 1) + 8 * (r >> 2) + 4 * (dt & 1) + (r & 3); }
 
-// Where a tile's operands are.
-template <int KB, int NI>
-__device__ __forceinline__ __bf16* key_tiles(const Args& a, int64_t tile, int hk) {
-  return a.keys + ((tile * a.Hk + hk) * 3) * (int64_t)(4 * KB * NI * kFrag);
-}
 template <typename T, bool BWD>
-constexpr int kTriSize = kTri * (NX + (BWD ? NX : kOutTerms<T>)) * kFrag;
+constexpr int kTriSize = kTri * (NX + (BWD ? 0 : kOutTerms<T>)) * kFrag;
 template <typename T, bool BWD>
 __device__ __forceinline__ __bf16* tri_tiles(const Args& a, int64_t tile, int h) {
   return a.tris + (tile * a.H + h) * (int64_t)kTriSize<T, BWD>;
 }
 __device__ __forceinline__ float* vec_of(const Args& a, int64_t tile, int h) {
   return a.vecs + (tile * a.H + h) * (int64_t)(V_COUNT * C);
+}
+
+// States, u and the gradient of R are kept for grads() as 16-bit planes, one per term, of 32
+// columns: rows are the columns, and in a row lie the channels (tokens) in order, in
+// chunks of eight.  So a wavefront that has 16 columns writes chunks, and the
+// transposing LDS read gives operands whose inner index is the column.  A row's
+// chunks are permuted by an exclusive or with its number, so that the 16 rows that
+// one such read takes lie in different banks.
+template <int KB>
+__device__ __forceinline__ int plane_swizzle(int row) {
+  const int a = (row >> 3) & 1;
+  return KB == 2 ? 2 * (((row >> 1) & 1) | a << 1) : KB == 4 ? 2 * ((row & 3) | a << 2) : 2 * a;
+}
+// Element of row `row`, channel (token) `at`, in a plane of 32 KB of them per row.
+template <int KB>
+__device__ __forceinline__ int plane_at(int row, int at) {
+  return row * 32 * KB + (((at >> 3) ^ plane_swizzle<KB>(row)) << 3) + (at & 7);
+}
+// Operand with rows 16 rt + lane % 16 of the channels (tokens), inner indices the 32 columns.
+template <int KB>
+__device__ __forceinline__ Terms<NX> load_plane(const __bf16* planes, int rt, int lane) {
+  const int j = lane & 15, row = 8 * (lane >> 4) + (j >> 2);
+  Terms<NX> r;
+#pragma unroll
+  for (int n = 0; n < NX; ++n) {
+    const __bf16* p = planes + n * 32 * 32 * KB;
+    const u32x2 a = read_transposed(p + plane_at<KB>(row, 16 * rt + 4 * (j & 3)));
+    const u32x2 b = read_transposed(p + plane_at<KB>(row + 4, 16 * rt + 4 * (j & 3)));
+    r.t[n] = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y));
+  }
+  return r;
+}
+// A wavefront's 16 columns (group cg) of `x`, rows in the order of registers, as terms to their planes.
+template <int KB>  // x: a state's terms
+__device__ __forceinline__ void keep_state(__bf16* planes, int cg, int m, int g, const Terms<NX> (&x)[KB]) {
+  const int row = 16 * (cg & 1) + m;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int n = 0; n < NX; ++n)
+      *reinterpret_cast<bf16x8*>(planes + n * 32 * 32 * KB + plane_at<KB>(row, 32 * kb + 8 * g)) = x[kb].t[n];
+}
+__device__ __forceinline__ void keep_rows(__bf16* planes, int cg, int m, int g, const Terms<NX> (&x)[2]) {
+  const int row = 16 * (cg & 1) + m;
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int n = 0; n < NX; ++n) {
+      const uint4 y = __builtin_bit_cast(uint4, x[kb].t[n]);
+      __bf16* p = planes + n * 32 * C;
+      *reinterpret_cast<u32x2*>(p + plane_at<2>(row, 32 * kb + 4 * g)) = u32x2{y.x, y.y};
+      *reinterpret_cast<u32x2*>(p + plane_at<2>(row, 32 * kb + 16 + 4 * g)) = u32x2{y.z, y.w};
+    }
+}
+// The planes of a tile, head and block of 32 columns.
+template <int KB>
+__device__ __forceinline__ int64_t planes_of(const Args& a, int64_t tile, int h, int block) {
+  return ((tile * a.H + h) * a.blocks + block) * (int64_t)(NX * 32 * 32 * KB);
 }
 
 template <int N>
@@ -127,23 +183,6 @@ __device__ __forceinline__ bf16x8 selector(int inner, int g) {
   return r;
 }
 
-// Tile f of the transpose of a chunk's rows, from their tiles in LDS (rows are channels, inner
-// indices tokens of half f % 2).
-template <int KB, int NI>
-__device__ __forceinline__ Terms<NI> transposed(const __bf16* tiles, int f, int lane) {
-  const int d = channel(f / 2, lane & 15), t0 = 32 * (f & 1) + 4 * (lane >> 4);
-  const int src = (d / 32) * NI * kFrag + (d & 7), sl = 16 * ((d >> 3) & 3);
-  Terms<NI> r;
-#pragma unroll
-  for (int j = 0; j < NI; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int t = t0 + (i & 3) + 16 * (i >> 2);
-      r.t[j][i] = tiles[(t >> 4) * KB * NI * kFrag + src + j * kFrag + (sl + (t & 15)) * 8];
-    }
-  return r;
-}
-
 // A barrier that orders LDS accesses only: loads from global memory stay in flight.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -161,7 +200,8 @@ __device__ __forceinline__ float fade(double x) {
 // prep: T of one chunk and value head (BWD: what the backward's products take)
 // --------------------------------------------------------------------------
 // Grid (tiles, H), four wavefronts; wavefront w has tokens 16w..16w+15 of the chunk.
-// Operand tiles of terms, forward: T and P.  BWD: T and P transposed, K, K transposed and Q transposed.
+// Forward: T and P, as operand tiles of terms.  BWD: T transposed, and what of the gradients does
+// not depend on a state: P' dO and scale Q' (e^G dO).
 //
 // log decays are added up in 64 bits: the sums over a chunk can be far larger than
 // the differences that count.  One below -128 is taken as -128: e^-128 is 0 in 32 bits,
@@ -170,7 +210,9 @@ template <typename T, int KB, bool BWD>
 __global__ __launch_bounds__(256) void prep(Args a) {
   constexpr int NI = kInputTerms<T>;
   constexpr int LD = C + 4;
-  __shared__ __bf16 kq[BWD ? 2 : 1][4 * KB * NI * kFrag];  // K and Q
+  constexpr int kKeys = 4 * KB * NI * kFrag, kQt = 4 * KB * NX * kFrag, kDo = 8 * NI * kFrag;
+  // K (and Q); BWD: later Q transposed and 64 columns of dO transposed
+  __shared__ __align__(16) __bf16 kq[!BWD ? kKeys : 2 * kKeys > kQt + kDo ? 2 * kKeys : kQt + kDo];
   __shared__ float As[C * LD], Ts[C * LD];
   __shared__ double Gs[C];
   __shared__ float bs[C];
@@ -229,29 +271,17 @@ __global__ __launch_bounds__(256) void prep(Args a) {
   for (int kb = 0; kb < KB; ++kb) {
     const int left = t < n ? a.Dk - 32 * kb - 8 * g : 0;
     kt[kb] = terms_of<T>(kr[kb], left);
-    store_terms<NI>(kq[0] + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
-    if constexpr (BWD) store_terms<NI>(kq[1] + (w * KB + kb) * NI * kFrag, lane, terms_of<T>(qr[kb], left));
+    store_terms<NI>(kq + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
+    if constexpr (BWD) store_terms<NI>(kq + kKeys + (w * KB + kb) * NI * kFrag, lane, terms_of<T>(qr[kb], left));
   }
   __syncthreads();
-  if constexpr (BWD) {
-    if (h % a.group == 0) {
-      __bf16* out = key_tiles<KB, NI>(a, tile, hk);
-      constexpr int kAll = 4 * KB * NI * kFrag;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) store_terms<NI>(out + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
-      for (int f = w; f < 4 * KB; f += 4)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          store_terms<NI>(out + (1 + x) * kAll + f * NI * kFrag, lane, transposed<KB, NI>(kq[x], f, lane));
-    }
-  }
   // A for tokens i of this wavefront, lane m = column j (read by rows below).
 #pragma unroll
   for (int jt = 0; jt < 4; ++jt) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (jt <= w) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) acc = product<2>(kt[kb], load_terms<NI>(kq[0] + (jt * KB + kb) * NI * kFrag, lane), acc);
+      for (int kb = 0; kb < KB; ++kb) acc = product<2>(kt[kb], load_terms<NI>(kq + (jt * KB + kb) * NI * kFrag, lane), acc);
       settle(acc);
     }
     const int j = 16 * jt + m;
@@ -261,9 +291,8 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       As[i * LD + j] = j < i ? bs[i] * fade(Gs[i] - Gs[j]) * acc[x] : 0.f;
     }
   }
+  Terms<BWD ? NX : 1> pt[2] = {};  // BWD: P transposed
   {  // P: rows i of this wavefront (BWD: transposed, rows j)
-    __bf16* tri = tri_tiles<T, BWD>(a, tile, h) + kTri * NX * kFrag;
-    constexpr int NO = BWD ? NX : kOutTerms<T>;
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
       if (BWD ? kb2 < w / 2 : kb2 > w / 2) continue;
@@ -272,7 +301,7 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       for (int kb = 0; kb < KB; ++kb) {
         Terms<NI> y[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) y[x] = load_terms<NI>(kq[BWD ? 1 : 0] + ((2 * kb2 + x) * KB + kb) * NI * kFrag, lane);
+        for (int x = 0; x < 2; ++x) y[x] = load_terms<NI>(kq + (BWD ? kKeys : 0) + ((2 * kb2 + x) * KB + kb) * NI * kFrag, lane);
         if constexpr (BWD)
           products<2>(y, kt[kb], p);
         else
@@ -286,7 +315,12 @@ __global__ __launch_bounds__(256) void prep(Args a) {
           const int other = 32 * kb2 + 16 * x + 4 * g + r, i = BWD ? other : t, j = BWD ? t : other;
           p[x][r] = j <= i ? a.scale * fade(Gs[i] - Gs[j]) * p[x][r] : 0.f;
         }
-      store_terms<NO>(tri + (BWD ? tri_upper(w, kb2) : tri_lower(w, kb2)) * NO * kFrag, lane, split<NO>(p[0], p[1]));
+      if constexpr (BWD) {
+        pt[kb2] = split<NX>(p[0], p[1]);
+      } else {
+        constexpr int NO = kOutTerms<T>;
+        store_terms<NO>(tri_tiles<T, false>(a, tile, h) + (kTri * NX + tri_lower(w, kb2) * NO) * kFrag, lane, split<NO>(p[0], p[1]));
+      }
     }
   }
   __syncthreads();
@@ -348,6 +382,83 @@ __global__ __launch_bounds__(256) void prep(Args a) {
     const int f = BWD ? tri_upper(w, kb2) : tri_lower(w, kb2);
     store_terms<NX>(tri_tiles<T, BWD>(a, tile, h) + f * NX * kFrag, lane, split<NX>(x[0], x[1]));
   }
+  if constexpr (BWD) {
+    __bf16 *Qt = kq, *Do = kq + kQt;
+    const f32x4 since = a.scale * f32x4{fade(Gs[16 * w + 4 * g]), fade(Gs[16 * w + 4 * g + 1]), fade(Gs[16 * w + 4 * g + 2]), fade(Gs[16 * w + 4 * g + 3])};
+    // Q transposed, rows in the order of a state's.
+    const bf16x8 ksel[2] = {selector(channel(0, m), g), selector(channel(1, m), g)};
+    const bf16x8 vsel[2] = {selector(m, g), selector(16 + m, g)};
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const Terms<NI> q = terms_of<T>(qr[kb], t < n ? a.Dk - 32 * kb - 8 * g : 0);
+      f32x4 y[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        y[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = NI - 1; j >= 0; --j) y[x] = mfma(q.t[j], ksel[x], y[x]);
+      }
+      settle(y);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const Terms<NX> e = split<NX>(y[x] * since, y[x]);
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+          const uint4 z = __builtin_bit_cast(uint4, e.t[j]);
+          *reinterpret_cast<u32x2*>(Qt + (((2 * kb + x) * 2 + (w >> 1)) * NX + j) * kFrag + lane * 8 + 4 * (w & 1)) = u32x2{z.x, z.y};
+        }
+      }
+    }
+    const T* obase = (const T*)a.d_o + at.rows.batch * a.dob + h * a.doh + row0 * a.don;
+    for (int c0 = 0; c0 < 16 * a.groups; c0 += 64) {
+      Raw8<T> raw[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) raw[b] = fetch8(obase, t * a.don + c0 + 32 * b + 8 * g, t < n ? a.Dv - c0 - 32 * b - 8 * g : 0);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const Terms<NI> o = terms_of<T>(raw[b], t < n ? a.Dv - c0 - 32 * b - 8 * g : 0);
+        f32x4 y[2 * NI];
+#pragma unroll
+        for (int x = 0; x < 2 * NI; ++x) y[x] = mfma(o.t[x % NI], vsel[x / NI], f32x4{0.f, 0.f, 0.f, 0.f});
+        settle(y);
+#pragma unroll
+        for (int x = 0; x < 2 * NI; ++x) {
+          const u32x2 r = {upper_halves(y[x][0], y[x][1]), upper_halves(y[x][2], y[x][3])};
+          *reinterpret_cast<u32x2*>(Do + (((2 * b + x / NI) * 2 + (w >> 1)) * NI + x % NI) * kFrag + lane * 8 + 4 * (w & 1)) = r;
+        }
+      }
+      __syncthreads();
+      const int64_t cg = (tile * a.H + h) * a.groups + (c0 >> 4);
+      const auto times_do = [&](const Terms<NX> (&x)[2], float* to, int64_t step) {
+        f32x4 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb2 = 0; kb2 < 2; ++kb2) {
+          Terms<NI> o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = load_terms<NI>(Do + (i * 2 + kb2) * NI * kFrag, lane);
+#pragma unroll
+          for (int ord = 2; ord >= 0; --ord)
+#pragma unroll
+            for (int j = 0; j < NX; ++j)
+              if (ord - j >= 0 && ord - j < NI)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = mfma(x[kb2].t[j], o[i].t[ord - j >= 0 && ord - j < NI ? ord - j : 0], y[i]);
+        }
+        settle(y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((c0 >> 4) + i < a.groups) *reinterpret_cast<f32x4*>(to + i * step) = y[i];
+      };
+      times_do(pt, a.ys + (cg * 4 + w) * 256 + lane * 4, 4 * 256);
+      for (int dt = w; dt < 2 * KB; dt += 4) {
+        const Terms<NX> q[2] = {load_terms<NX>(Qt + (dt * 2) * NX * kFrag, lane), load_terms<NX>(Qt + (dt * 2 + 1) * NX * kFrag, lane)};
+        times_do(q, a.zs + (cg * 2 * KB + dt) * 256 + lane * 4, 2 * KB * 256);
+      }
+      __syncthreads();
+    }
+  }
 }
 
 // --------------------------------------------------------------------------
@@ -395,7 +506,12 @@ __device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, 
     o = group_sum(o);
     if (g == 0 && col < a.Dv) {
       ((T*)a.o)[rows.batch * a.ob + h * a.oh + (row0 + t) * a.on + col] = (T)(a.scale * o);
-      if (SAVE) a.us[(((tile * a.H + h) * a.groups + col / 16) * 4 + t / 16) * 256 + (16 * ((t & 15) / 4) + (col & 15)) * 4 + (t & 3)] = u;
+      if (SAVE) {
+        const float y[8] = {u};
+        const Terms<NX> e = split<NX>(y);
+#pragma unroll
+        for (int j = 0; j < NX; ++j) a.us[planes_of<2>(a, tile, h, col >> 5) + j * 32 * C + plane_at<2>(col & 31, t)] = e.t[j][0];
+      }
     }
   }
 }
@@ -428,7 +544,8 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   const int col0 = blockIdx.z * 16 * NW;
   if (wave < NW) {
     const int col = col0 + 16 * wave + m;
-    const bool in = col < a.Dv, any = col0 + 16 * wave < a.Dv;
+    const int cg = (col0 >> 4) + wave;
+    const bool in = col < a.Dv, any = cg < a.groups;
     f32x4 S[2 * KB];
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt)
@@ -440,14 +557,9 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     if (nch) lds_barrier();
     for (int64_t c = 0; c < nch; ++c) {
       const int64_t tile = tile0 + c;
-      const int64_t cg = (tile * a.H + h) * a.groups + (col0 >> 4) + wave;
       const float* vec = vecs[c & 1];
       f32x4 X[4];
       if (any) {
-        if (SAVE) {
-#pragma unroll
-          for (int dt = 0; dt < 2 * KB; ++dt) *reinterpret_cast<f32x4*>(a.states + (cg * 2 * KB + dt) * 256 + lane * 4) = S[dt];
-        }
         Terms<NX> s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -456,6 +568,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
           for (int j = 0; j < NO; ++j)
             *reinterpret_cast<bf16x8*>(Sf + ((wave * KB + kb) * NO + j) * kFrag + lane * 8) = s[kb].t[j];
         }
+        if (SAVE) keep_state<KB>(a.states + planes_of<KB>(a, tile, h, cg >> 1), cg, m, g, s);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) X[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -504,8 +617,8 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
                                       tile, S);
         } else {
           if (SAVE) {
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) *reinterpret_cast<f32x4*>(a.us + (cg * 4 + mt) * 256 + lane * 4) = U[mt];
+            const Terms<NX> u[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
+            keep_rows(a.us + planes_of<2>(a, tile, h, cg >> 1), cg, m, g, u);
           }
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
@@ -681,8 +794,9 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
 // Backward.  With dS the gradient of the state at a chunk's end (P with scale):
 //     dU = P' dO + e^{G_64 - G} (K dS)          dR = T' dU
 //     dS <- e^{G_64} dS + scale Q' (e^G dO) - K' (b e^G dR)
-// chain_back() goes through the chunks from the last to the first as chain() does and
-// leaves dR and each chunk's dS; grads() then has everything of its chunk:
+// prep() leaves P' dO and scale Q' (e^G dO) of every chunk; chain_back() goes through the chunks
+// from the last to the first as chain() does and leaves dR and each chunk's dS;
+// grads() then has everything of its chunk:
 //     dq = scale e^G (S dO) + (dP o D) K           dP_ij = dO_i.u_j,  D_ij = scale e^{G_i - G_j}, j <= i
 //     dk = b rho + kw                              dA_ij = -dR_i.u_j (over b_i: below)
 //     rho_i = -e^{G_i} S dR_i + sum_{j<i} dA_ij e^{G_i-G_j} k_j
@@ -693,136 +807,184 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
 //     dg_i = sum of dG_i.. to the chunk's end
 // --------------------------------------------------------------------------
 template <typename T, int KB>
-__global__ __launch_bounds__(256) void chain_back(Args a) {
-  constexpr int NI = kInputTerms<T>;
+__global__ __launch_bounds__(512) void chain_back(Args a) {
+  constexpr int NI = kInputTerms<T>, NW = 4;
+  __shared__ __bf16 Kf[4 * KB * NI * kFrag], Kt[4 * KB * NI * kFrag], Tf[kTri * NX * kFrag];
+  __shared__ float vecs[2][V_CHAIN * C];
   const int64_t seq = blockIdx.x;
   const int h = blockIdx.y, hk = h / a.group;
-  const int wave = blockIdx.z * (blockDim.x / 64) + wave_index();
-  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  if (16 * wave >= a.Dv) return;
-  const int col = 16 * wave + m;
-  const bool in = col < a.Dv;
+  const int wave = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const Rows rows = rows_of(a.cu, seq, a.N);
   const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), nch = (rows.n + C - 1) / C;
-  f32x4 S[2 * KB];
-#pragma unroll
-  for (int dt = 0; dt < 2 * KB; ++dt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = channel(dt, 4 * g + i);
-      S[dt][i] = a.d_final && in && d < a.Dk ? a.d_final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
-    }
-  for (int64_t c = nch - 1; c >= 0; --c) {
-    const int64_t tile = tile0 + c, row0 = rows.first + c * C;
-    const int n = rows.n - c * C < C ? (int)(rows.n - c * C) : C;
-    const int64_t cg = (tile * a.H + h) * a.groups + wave;
-#pragma unroll
-    for (int dt = 0; dt < 2 * KB; ++dt) *reinterpret_cast<f32x4*>(a.dstates + (cg * 2 * KB + dt) * 256 + lane * 4) = S[dt];
-    constexpr int kAll = 4 * KB * NI * kFrag;
-    const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
-    const __bf16* tri = tri_tiles<T, true>(a, tile, h);
-    const float* vec = vec_of(a, tile, h);
-    f32x4 dO[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * mt + 4 * g + i;
-        dO[mt][i] =
-            t < n && in ? (float)((const T*)a.d_o)[rows.batch * a.dob + h * a.doh + (row0 + t) * a.don + col] : 0.f;
-      }
-    const Terms<NI> o[2] = {split<NI>(dO[0], dO[1]), split<NI>(dO[2], dO[3])};
-    Terms<NX> s[KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
-    f32x4 U[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) x = product<2>(load_terms<NI>(kf + (mt * KB + kb) * NI * kFrag, lane), s[kb], x);
-      settle(x);
-      x *= *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
-#pragma unroll
-      for (int kb = mt / 2; kb < 2; ++kb)
-        x = product<2>(load_terms<NX>(tri + (kTri + tri_upper(mt, kb)) * NX * kFrag, lane), o[kb], x);
-      U[mt] = x;
-    }
-    settle(U);
-    const Terms<NX> u[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
-    f32x4 R[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = mt / 2; kb < 2; ++kb) x = product<2>(load_terms<NX>(tri + tri_upper(mt, kb) * NX * kFrag, lane), u[kb], x);
-      settle(x);
-      R[mt] = x;
-      *reinterpret_cast<f32x4*>(a.drs + (cg * 4 + mt) * 256 + lane * 4) = x;
-      const f32x4 b = *reinterpret_cast<const f32x4*>(vec + V_BETA * C + 16 * mt + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * mt + 4 * g + i;
-        if (in) {
-          if (t < n) ((T*)a.dv)[rows.batch * a.dvb + h * a.dvh + (row0 + t) * a.dvn + col] = (T)(b[i] * x[i]);
-        }
-      }
-    }
-    const float whole = vec[V_SINCE * C + C - 1];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      R[mt] *= *reinterpret_cast<const f32x4*>(vec + V_BG * C + 16 * mt + 4 * g);
-      R[mt] = -R[mt];
-      dO[mt] *= a.scale * *reinterpret_cast<const f32x4*>(vec + V_SINCE * C + 16 * mt + 4 * g);
-    }
-    const Terms<NX> r[2] = {split<NX>(R[0], R[1]), split<NX>(R[2], R[3])};
-    const Terms<NX> e[2] = {split<NX>(dO[0], dO[1]), split<NX>(dO[2], dO[3])};
-#pragma unroll
-    for (int dt = 0; dt < 2 * KB; ++dt) {
-      S[dt] *= whole;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        S[dt] = product<2>(load_terms<NI>(kf + kAll + (dt * 2 + kb) * NI * kFrag, lane), r[kb], S[dt]);
-        S[dt] = product<2>(load_terms<NI>(kf + 2 * kAll + (dt * 2 + kb) * NI * kFrag, lane), e[kb], S[dt]);
-      }
-    }
-    settle(S);
-  }
-  if (a.d_init) {
+  if (wave < NW) {
+    const int cg = blockIdx.z * NW + wave, col = 16 * cg + m;
+    const bool in = col < a.Dv, any = cg < a.groups;
+    f32x4 S[2 * KB], Y[4], Z[2 * KB];
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = channel(dt, 4 * g + i);
-        if (in && d < a.Dk) a.d_init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+        S[dt][i] = a.d_final && in && d < a.Dk ? a.d_final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
       }
+    const auto fetch = [&](int64_t c) {
+      const int64_t at = ((tile0 + c) * a.H + h) * a.groups + (any ? cg : 0);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) Y[mt] = *reinterpret_cast<const f32x4*>(a.ys + (at * 4 + mt) * 256 + lane * 4);
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt) Z[dt] = *reinterpret_cast<const f32x4*>(a.zs + (at * 2 * KB + dt) * 256 + lane * 4);
+    };
+    if (nch) {
+      fetch(nch - 1);
+      lds_barrier();
+    }
+    for (int64_t c = nch - 1; c >= 0; --c) {
+      const int64_t tile = tile0 + c;
+      const float* vec = vecs[c & 1];
+      f32x4 X[4];
+      if (any) {
+        Terms<NX> s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+        keep_state<KB>(a.dstates + planes_of<KB>(a, tile, h, cg >> 1), cg, m, g, s);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) X[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          Terms<NI> k[4];
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) k[mt] = load_terms<NI>(Kf + (mt * KB + kb) * NI * kFrag, lane);
+          products<2>(k, s[kb], X);
+        }
+        settle(X);
+      }
+      lds_barrier();
+      if (any) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          const f32x4 left = *reinterpret_cast<const f32x4*>(vec + V_LEFT * C + 16 * mt + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) X[mt][i] = fmaf(left[i], X[mt][i], Y[mt][i]);
+        }
+        const float whole = vec[V_SINCE * C + C - 1];
+#pragma unroll
+        for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(whole, S[dt][i], Z[dt][i]);
+        if (c) fetch(c - 1);
+        const Terms<NX> u[2] = {split<NX>(X[0], X[1]), split<NX>(X[2], X[3])};
+        f32x4 R[4];
+        {
+          Terms<NX> x[4], y[2];
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            R[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            x[mt] = load_terms<NX>(Tf + tri_upper(mt, 1) * NX * kFrag, lane);
+          }
+          products<2>(x, u[1], R);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) y[mt] = load_terms<NX>(Tf + tri_upper(mt, 0) * NX * kFrag, lane);
+          products<2>(y, u[0], R);
+        }
+        settle(R);
+        {
+          const Terms<NX> r[2] = {split<NX>(R[0], R[1]), split<NX>(R[2], R[3])};
+          keep_rows(a.drs + planes_of<2>(a, tile, h, cg >> 1), cg, m, g, r);
+        }
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) R[mt] *= -*reinterpret_cast<const f32x4*>(vec + V_BG * C + 16 * mt + 4 * g);
+        const Terms<NX> r[2] = {split<NX>(R[0], R[1]), split<NX>(R[2], R[3])};
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          Terms<NI> k[2 * KB];
+#pragma unroll
+          for (int dt = 0; dt < 2 * KB; ++dt) k[dt] = load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane);
+          products<2>(k, r[kb], S);
+        }
+        settle(S);
+      }
+      lds_barrier();
+    }
+    if (a.d_init) {
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = channel(dt, 4 * g + i);
+          if (in && d < a.Dk) a.d_init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] = S[dt][i];
+        }
+    }
+    return;
+  }
+  if (!nch) return;
+  // A feeder: tokens 16w + m of each chunk, as in chain().
+  const int w = wave - NW, t = 16 * w + m, ft = threadIdx.x - 64 * NW;
+  constexpr int TP = (kTri * NX + 3) / 4;
+  const T* kbase = (const T*)a.k + rows.batch * a.kb + hk * a.kh + rows.first * a.kn;
+  Raw8<T> kr[KB];
+  bf16x8 tr[TP];
+  f32x4 er;
+  const auto left_of = [&](int64_t c) { return c * C + t < rows.n ? a.Dk - 8 * g : 0; };
+  const auto fetch = [&](int64_t c) {
+    const int dk = left_of(c);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) kr[kb] = fetch8(kbase, (c * C + t) * a.kn + 32 * kb + 8 * g, dk - 32 * kb);
+    const __bf16* tri = tri_tiles<T, true>(a, tile0 + c, h) + w * kFrag + lane * 8;
+#pragma unroll
+    for (int x = 0; x < TP; ++x)
+      if (4 * x + 4 <= kTri * NX || w + 4 * x < kTri * NX) tr[x] = *reinterpret_cast<const bf16x8*>(tri + 4 * x * kFrag);
+    er = *reinterpret_cast<const f32x4*>(vec_of(a, tile0 + c, h) + (ft % (V_CHAIN * C / 4)) * 4);
+  };
+  Terms<NI> kt[KB];
+  const auto put_keys = [&](int64_t c) {
+    const int dk = left_of(c);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      kt[kb] = terms_of<T>(kr[kb], dk - 32 * kb);
+      store_terms<NI>(Kf + (w * KB + kb) * NI * kFrag, lane, kt[kb]);
+    }
+    if (ft < V_CHAIN * C / 4) *reinterpret_cast<f32x4*>(vecs[c & 1] + ft * 4) = er;
+  };
+  const bf16x8 ksel[2] = {selector(channel(0, m), g), selector(channel(1, m), g)};
+  fetch(nch - 1);
+  put_keys(nch - 1);
+  lds_barrier();
+  for (int64_t c = nch - 1; c >= 0; --c) {
+#pragma unroll
+    for (int x = 0; x < TP; ++x)
+      if (4 * x + 4 <= kTri * NX || w + 4 * x < kTri * NX) *reinterpret_cast<bf16x8*>(Tf + (w + 4 * x) * kFrag + lane * 8) = tr[x];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x4 y[2 * NI];
+#pragma unroll
+      for (int x = 0; x < 2 * NI; ++x) y[x] = mfma(kt[kb].t[x % NI], ksel[x / NI], f32x4{0.f, 0.f, 0.f, 0.f});
+      settle(y);
+#pragma unroll
+      for (int x = 0; x < 2 * NI; ++x) {
+        const u32x2 r = {upper_halves(y[x][0], y[x][1]), upper_halves(y[x][2], y[x][3])};
+        *reinterpret_cast<u32x2*>(Kt + (((2 * kb + x / NI) * 2 + (w >> 1)) * NI + x % NI) * kFrag + lane * 8 + 4 * (w & 1)) = r;
+      }
+    }
+    if (c) fetch(c - 1);
+    lds_barrier();
+    if (c) put_keys(c - 1);
+    lds_barrier();
   }
 }
 
-// One lane's eight values of a row, channels k0 + 8g.., of `width`.
-template <typename T>
-__device__ __forceinline__ void load8(const T* base, int64_t at, int k0, int g, int width, float (&x)[8]) {
-  const int d = k0 + 8 * g;
-  const Raw8<T> y = fetch8(base, at + d, width - d);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = width - d > 0 ? (float)y[i] : 0.f;
-}
-
-// Row r, columns c0 + 8g.. of a matrix that chain() or chain_back() kept as it lay in
-// registers, `tiles` tiles of 16 rows for each of the 16-column groups.
-__device__ __forceinline__ void load_kept(const float* x, int tiles, int r, int c0, int g, int groups, float (&y)[8]) {
-  const int cg = c0 / 16 + (g >> 1);
-  const float* p = x + ((cg < groups ? cg : 0) * tiles + r / 16) * 256 + (16 * ((r & 15) / 4) + 8 * (g & 1)) * 4 + (r & 3);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = cg < groups ? p[4 * i] : 0.f;
-}
-
-// Grid (tiles, Hk), four wavefronts; wavefront w has tokens 16w..16w+15, lane m the token
-// 16w + m, and channels 4g.. of each 16-channel tile: no product crosses wavefronts.
-template <typename T, int KB>
+// Grid (tiles, Hk), four wavefronts; wavefront w has tokens 16w..16w+15, lane m the token 16w + m, and
+// channels 4g.. of each 16-channel tile: no product's result crosses wavefronts.  First the
+// products over v's columns, 32 at a time (their planes go to LDS as they lie), then
+// those over the chunk's tokens, whose factors dO_i.u_j and dR_i.u_j are computed
+// both ways round, so that either is an operand as it stands.
+template <typename T, int KB, bool GROUPED>
 __global__ __launch_bounds__(256) void grads(Args a) {
   constexpr int NI = kInputTerms<T>;
-  constexpr int kAll = 4 * KB * NI * kFrag;
+  constexpr int SP = NX * 32 * 32 * KB, UP = NX * 32 * C, kKt = 4 * KB * NI * kFrag;
+  constexpr int kPlanes = 2 * SP + 2 * UP + 4 * NI * kFrag;
+  __shared__ __align__(16) __bf16 lds[kPlanes > 2 * kKt ? kPlanes : 2 * kKt];
+  __bf16 *Sp = lds, *dSp = lds + SP, *Up = lds + 2 * SP, *Rp = Up + UP, *Of = Rp + UP;  // planes, and rows of dO
+  __bf16 *Kt = lds, *Qt = lds + kKt;                                                    // later: K and Q transposed
   __shared__ float dGs[C], ends[4];
   const int64_t tile = blockIdx.x;
   const int hk = blockIdx.y;
@@ -839,15 +1001,19 @@ __global__ __launch_bounds__(256) void grads(Args a) {
   const int n = left_rows < C ? (int)left_rows : C;
   const int64_t row0 = at.rows.first + at.index * C, bt = at.rows.batch;
   const int t = 16 * w + m;
-  const __bf16* kf = key_tiles<KB, NI>(a, tile, hk);
-  f32x4 dq[2 * KB], dk[2 * KB];
+  const T* kbase = (const T*)a.k + bt * a.kb + hk * a.kh + row0 * a.kn;
+  const T* qbase = (const T*)a.q + bt * a.qb + hk * a.qh + row0 * a.qn;
+  const bf16x8 sel[2] = {selector(m, g), selector(16 + m, g)};
+  f32x4 dq[GROUPED ? 2 * KB : 1], dk[GROUPED ? 2 * KB : 1];
+  if (GROUPED) {
 #pragma unroll
-  for (int dt = 0; dt < 2 * KB; ++dt) dq[dt] = dk[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int dt = 0; dt < 2 * KB; ++dt) dq[GROUPED ? dt : 0] = dk[GROUPED ? dt : 0] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
     const float* vec = vec_of(a, tile, h);
-    const int64_t cg = (tile * a.H + h) * a.groups;
-    const float *St = a.states + cg * 2 * KB * 256, *dSt = a.dstates + cg * 2 * KB * 256;
-    const float *Us = a.us + cg * 4 * 256, *Rs = a.drs + cg * 4 * 256;
+    const T* obase = (const T*)a.d_o + bt * a.dob + h * a.doh + row0 * a.don;
+    const T* vbase = (const T*)a.v + bt * a.vb + h * a.vh + row0 * a.vn;
+    const float bt_ = vec[V_BETA * C + t];
     f32x4 hq[2 * KB], rho[2 * KB], kw[2 * KB];
     f32x4 E1[4], E2[4], F1[4], F2[4];  // dO_i.u_j and dR_i.u_j: lane = i, rows j <= i; lane = j, rows i >= j
 #pragma unroll
@@ -855,65 +1021,96 @@ __global__ __launch_bounds__(256) void grads(Args a) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) E1[x] = E2[x] = F1[x] = F2[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     float db = 0.f, ss = 0.f;
-    for (int c0 = 0; c0 < a.Dv; c0 += 32) {
-      float xo[8], xr[8], xu[8], xv[8];
-      load8((const T*)a.d_o + bt * a.dob + h * a.doh + row0 * a.don, t * a.don, c0, g, t < n ? a.Dv : 0, xo);
-      load8((const T*)a.v + bt * a.vb + h * a.vh + row0 * a.vn, t * a.vn, c0, g, t < n ? a.Dv : 0, xv);
-      load_kept(Rs, 4, t, c0, g, t < n ? a.groups : 0, xr);
-      load_kept(Us, 4, t, c0, g, t < n ? a.groups : 0, xu);
+    for (int b = 0; b < a.blocks; ++b) {
+      const int c0 = 32 * b, dv = t < n ? a.Dv - c0 - 8 * g : 0;
+      __syncthreads();  // what lds held is read
+      const Raw8<T> oraw = fetch8(obase, t * a.don + c0 + 8 * g, dv), vraw = fetch8(vbase, t * a.vn + c0 + 8 * g, dv);
+      const int64_t so = planes_of<KB>(a, tile, h, b), uo = planes_of<2>(a, tile, h, b);
+      constexpr int SN = SP / kFrag, UN = UP / kFrag;  // copies of 1 KiB
+      for (int i = w; i < SN; i += 4) {
+        copy_to_lds(a.states + so + i * kFrag + lane * 8, Sp + i * kFrag);
+        copy_to_lds(a.dstates + so + i * kFrag + lane * 8, dSp + i * kFrag);
+      }
+      for (int i = w; i < UN; i += 4) {
+        copy_to_lds(a.us + uo + i * kFrag + lane * 8, Up + i * kFrag);
+        copy_to_lds(a.drs + uo + i * kFrag + lane * 8, Rp + i * kFrag);
+      }
+      const Terms<NI> o = terms_of<T>(oraw, dv);
+      store_terms<NI>(Of + w * NI * kFrag, lane, o);
+      lds_copies_done();
+      __syncthreads();
+      const Terms<NX> u = load_plane<2>(Up, w, lane), r = load_plane<2>(Rp, w, lane);
+      {
+        float x[8];
+        Raw8<T> dvs;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) db = fmaf(xr[i], xv[i], db);
-      const Terms<NI> o = split<NI>(xo);
-      const Terms<NX> r = split<NX>(xr), u = split<NX>(xu);
+        for (int i = 0; i < 8; ++i) {
+          x[i] = t < n ? ((float)r.t[2][i] + (float)r.t[1][i]) + (float)r.t[0][i] : 0.f;
+          db = fmaf(x[i], dv > 0 ? (float)vraw[i] : 0.f, db);
+          dvs[i] = (T)(bt_ * x[i]);
+        }
+        if (dv > 0)
+          *reinterpret_cast<Raw8<T>*>((T*)a.dv + bt * a.dvb + h * a.dvh + (row0 + t) * a.dvn + c0 + 8 * g) = dvs;
+      }
 #pragma unroll
       for (int dt = 0; dt < 2 * KB; ++dt) {
-        const int d = 16 * dt + m;  // as kept
-        float xs[8], xd[8];
-        load_kept(St, 2 * KB, d, c0, g, a.groups, xs);
-        load_kept(dSt, 2 * KB, d, c0, g, a.groups, xd);
-        if (dt % 4 == w) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(xs[i], xd[i], ss);
-        }
-        const Terms<NX> s = split<NX>(xs), ds = split<NX>(xd);
+        const Terms<NX> s = load_plane<KB>(Sp, dt, lane), ds = load_plane<KB>(dSp, dt, lane);
         hq[dt] = product<2>(s, o, hq[dt]);
         rho[dt] = product<2>(s, r, rho[dt]);
         kw[dt] = product<2>(ds, u, kw[dt]);
+        if (dt % 4 == w) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            ss = fmaf(((float)s.t[2][i] + (float)s.t[1][i]) + (float)s.t[0][i],
+                      ((float)ds.t[2][i] + (float)ds.t[1][i]) + (float)ds.t[0][i], ss);
+        }
+        settle(hq[dt]), settle(rho[dt]), settle(kw[dt]);
       }
-      settle(hq), settle(rho), settle(kw);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int y = 16 * x + m;
         if (x <= w) {
-          float z[8];
-          load_kept(Us, 4, y, c0, g, y < n ? a.groups : 0, z);
-          const Terms<NX> uj = split<NX>(z);
+          const Terms<NX> uj = load_plane<2>(Up, x, lane);
           E1[x] = product<2>(uj, o, E1[x]);
           E2[x] = product<2>(uj, r, E2[x]);
           settle(E1[x]), settle(E2[x]);
         }
         if (x >= w) {
-          float z[8];
-          load8((const T*)a.d_o + bt * a.dob + h * a.doh + row0 * a.don, y * a.don, c0, g, y < n ? a.Dv : 0, z);
-          F1[x] = product<2>(split<NI>(z), u, F1[x]);
-          load_kept(Rs, 4, y, c0, g, y < n ? a.groups : 0, z);
-          F2[x] = product<2>(split<NX>(z), u, F2[x]);
+          F1[x] = product<2>(load_terms<NI>(Of + x * NI * kFrag, lane), u, F1[x]);
+          F2[x] = product<2>(load_plane<2>(Rp, x, lane), u, F2[x]);
           settle(F1[x]), settle(F2[x]);
         }
       }
     }
-    const float Gt = vec[V_G * C + t], Gl = vec[V_GLOW * C + t], bt_ = vec[V_BETA * C + t];
+    // K and Q transposed
+    __syncthreads();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int d = 32 * kb + 8 * g, left = t < n ? a.Dk - d : 0;
+      const Terms<NI> kt = terms_of<T>(fetch8(kbase, t * a.kn + d, left), left), qt = terms_of<T>(fetch8(qbase, t * a.qn + d, left), left);
+      f32x4 y[4 * NI];
+#pragma unroll
+      for (int x = 0; x < 2 * NI; ++x) {
+        y[x] = mfma(kt.t[x % NI], sel[x / NI], f32x4{0.f, 0.f, 0.f, 0.f});
+        y[2 * NI + x] = mfma(qt.t[x % NI], sel[x / NI], f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+      settle(y);
+#pragma unroll
+      for (int x = 0; x < 4 * NI; ++x) {
+        const int z = x % (2 * NI);
+        __bf16* to = (x < 2 * NI ? Kt : Qt) + (((2 * kb + z / NI) * 2 + (w >> 1)) * NI + z % NI) * kFrag + lane * 8 + 4 * (w & 1);
+        *reinterpret_cast<u32x2*>(to) = u32x2{upper_halves(y[x][0], y[x][1]), upper_halves(y[x][2], y[x][3])};
+      }
+    }
+    const float Gt = vec[V_G * C + t], Gl = vec[V_GLOW * C + t];
     const float since = vec[V_SINCE * C + t], left = vec[V_LEFT * C + t], whole = vec[V_SINCE * C + C - 1];
     // k.(the state's part of kw), q.dq, k.rho, k.kw
     float kend = 0.f, qq = 0.f, kr = 0.f, kk = 0.f;
-    const T* kbase = (const T*)a.k + bt * a.kb + hk * a.kh + row0 * a.kn;
-    const T* qbase = (const T*)a.q + bt * a.qb + hk * a.qh + row0 * a.qn;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
       hq[dt] *= a.scale * since;
       rho[dt] *= -since;
       kw[dt] *= left;
-      const f32x4 k = load4(kbase, t * a.kn + channel(dt, 4 * g), t < n ? a.Dk - channel(dt, 4 * g) : 0);
+      const f32x4 k = load4(kbase, t * a.kn + 16 * dt + 4 * g, t < n ? a.Dk - 16 * dt - 4 * g : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) kend = fmaf(k[i], kw[dt][i], kend);
     }
@@ -933,6 +1130,7 @@ __global__ __launch_bounds__(256) void grads(Args a) {
         F2[x][i] = y > t ? -by[i] * fj * F2[x][i] : 0.f;
       }
     }
+    __syncthreads();
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       const bool lo = kb <= w / 2, hi = kb >= w / 2;
@@ -940,31 +1138,41 @@ __global__ __launch_bounds__(256) void grads(Args a) {
       const Terms<NX> f1 = split<NX>(F1[2 * kb], F1[2 * kb + 1]), f2 = split<NX>(F2[2 * kb], F2[2 * kb + 1]);
 #pragma unroll
       for (int dt = 0; dt < 2 * KB; ++dt) {
-        const Terms<NI> kT = load_terms<NI>(kf + kAll + (dt * 2 + kb) * NI * kFrag, lane);
+        const Terms<NI> kT = load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane);
         if (lo) {
           hq[dt] = product<2>(kT, e1, hq[dt]);
           rho[dt] = product<2>(kT, e2, rho[dt]);
           settle(hq[dt]), settle(rho[dt]);
         }
         if (hi) {
-          const Terms<NI> qT = load_terms<NI>(kf + 2 * kAll + (dt * 2 + kb) * NI * kFrag, lane);
-          kw[dt] = product<2>(qT, f1, kw[dt]);
+          kw[dt] = product<2>(load_terms<NI>(Qt + (dt * 2 + kb) * NI * kFrag, lane), f1, kw[dt]);
           kw[dt] = product<2>(kT, f2, kw[dt]);
           settle(kw[dt]);
         }
       }
     }
+    T* dqrow = (T*)a.dq + bt * a.dqb + hk * a.dqh + (row0 + t) * a.dqn;
+    T* dkrow = (T*)a.dk + bt * a.dkb + hk * a.dkh + (row0 + t) * a.dkn;
+    const bool done = !GROUPED || h + 1 == (hk + 1) * a.group;
 #pragma unroll
     for (int dt = 0; dt < 2 * KB; ++dt) {
-      const f32x4 k = load4(kbase, t * a.kn + channel(dt, 4 * g), t < n ? a.Dk - channel(dt, 4 * g) : 0);
-      const f32x4 q = load4(qbase, t * a.qn + channel(dt, 4 * g), t < n ? a.Dk - channel(dt, 4 * g) : 0);
+      const int d = 16 * dt + 4 * g, ok = t < n ? a.Dk - d : 0;
+      const f32x4 k = load4(kbase, t * a.kn + d, ok), q = load4(qbase, t * a.qn + d, ok);
+      f32x4 dqs = hq[dt], dks;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         qq = fmaf(q[i], hq[dt][i], qq);
         kr = fmaf(k[i], rho[dt][i], kr);
         kk = fmaf(k[i], kw[dt][i], kk);
-        dq[dt][i] += hq[dt][i];
-        dk[dt][i] += fmaf(bt_, rho[dt][i], kw[dt][i]);
+        dks[i] = fmaf(bt_, rho[dt][i], kw[dt][i]);
+      }
+      if (GROUPED) {
+        dqs = dq[GROUPED ? dt : 0] += dqs;
+        dks = dk[GROUPED ? dt : 0] += dks;
+      }
+      if (done && ok > 0) {
+        store4(dqrow + d, dqs);
+        store4(dkrow + d, dks);
       }
     }
     kend = group_sum(kend), qq = group_sum(qq), kr = group_sum(kr), kk = group_sum(kk), db = group_sum(db);
@@ -975,13 +1183,12 @@ __global__ __launch_bounds__(256) void grads(Args a) {
       ss += __shfl_xor(ss, x);
     }
     ss = group_sum(ss);
-    __syncthreads();  // dGs and ends of the head before are read
     if (g == 0) {
       dGs[t] = qq + bt_ * kr - kk;
       if (t < n) a.dbeta[(bt * a.H + h) * a.N + row0 + t] = db + kr;
     }
     if (lane == 0) ends[w] = kend + whole * ss;
-    __syncthreads();
+    __syncthreads();  // (and one before they are written again: the next head's blocks begin with it)
     if (w == 0) {
       float x = dGs[lane];
 #pragma unroll
@@ -990,17 +1197,6 @@ __global__ __launch_bounds__(256) void grads(Args a) {
         if (lane + d < 64) x += y;
       }
       if (lane < n) a.dg[(bt * a.H + h) * a.N + row0 + lane] = x + ((ends[0] + ends[1]) + (ends[2] + ends[3]));
-    }
-  }
-  if (t < n) {
-    T* dqrow = (T*)a.dq + bt * a.dqb + hk * a.dqh + (row0 + t) * a.dqn;
-    T* dkrow = (T*)a.dk + bt * a.dkb + hk * a.dkh + (row0 + t) * a.dkn;
-#pragma unroll
-    for (int dt = 0; dt < 2 * KB; ++dt) {
-      const int d = channel(dt, 4 * g);
-      if (d >= a.Dk) continue;
-      store4(dqrow + d, dq[dt]);
-      store4(dkrow + d, dk[dt]);
     }
   }
 }
@@ -1119,19 +1315,22 @@ int64_t tiles_of(const kdelta_problem* p) {
 
 int input_terms(int dtype) { return dtype == KDECAY_BF16 ? 1 : dtype == KDECAY_F16 ? 2 : 3; }
 
+int64_t blocks_of(const kdelta_problem* p) { return (p->Dv + 31) / 32; }
+
 struct Sizes {  // bytes
-  size_t inv, keys, tris, vecs, dstates, drs;  // inv: the forward's T and P
+  size_t vecs, tris, back_tris, ys, zs, states, rows;
 };
 
 Sizes sizes_of(const kdelta_problem* p) {
-  const size_t tiles = tiles_of(p), KB = (p->Dk + 31) / 32, NI = input_terms(p->dtype), groups = (p->Dv + 15) / 16;
+  const size_t heads = (size_t)tiles_of(p) * p->H, KB = (p->Dk + 31) / 32, blocks = blocks_of(p);
   Sizes s;
-  s.inv = up256(tiles * p->H * kTri * (NX + (p->dtype == KDECAY_F32 ? 3 : 2)) * kFrag * 2);
-  s.keys = up256(tiles * p->Hk * 3 * 4 * KB * NI * kFrag * 2);
-  s.tris = up256(tiles * p->H * kTri * 2 * NX * kFrag * 2);
-  s.vecs = up256(tiles * p->H * V_COUNT * C * 4);
-  s.dstates = up256(tiles * p->H * groups * 2 * KB * 256 * 4);
-  s.drs = up256(tiles * p->H * groups * 4 * 256 * 4);
+  s.vecs = up256(heads * V_COUNT * C * 4);
+  s.tris = up256(heads * kTri * (NX + (p->dtype == KDECAY_F32 ? 3 : 2)) * kFrag * 2);
+  s.back_tris = up256(heads * kTri * NX * kFrag * 2);
+  s.ys = up256(heads * 2 * blocks * 4 * 256 * 4);
+  s.zs = up256(heads * 2 * blocks * 2 * KB * 256 * 4);
+  s.states = up256(heads * blocks * NX * 32 * 32 * KB * 2);
+  s.rows = up256(heads * blocks * NX * 32 * C * 2);
   return s;
 }
 
@@ -1159,7 +1358,7 @@ int check(const kdelta_problem* p) {
   return check_rows(p->v, p->v_strides, p->dtype, "v");
 }
 
-Args args_of(const kdelta_problem* p, void* workspace, bool backward) {
+Args args_of(const kdelta_problem* p, void* workspace, const float* saved, bool backward) {
   Args a = {};
   a.q = p->q, a.k = p->k, a.v = p->v, a.g = p->g, a.beta = p->beta, a.cu = p->cu_seqlens, a.init = p->init;
   a.qb = p->q_strides[0], a.qh = p->q_strides[1], a.qn = p->q_strides[2];
@@ -1170,18 +1369,21 @@ Args args_of(const kdelta_problem* p, void* workspace, bool backward) {
   a.N = p->N, a.sequences = p->sequences, a.tiles = tiles_of(p);
   a.Hk = (int)p->Hk, a.H = (int)p->H, a.Dk = (int)p->Dk, a.Dv = (int)p->Dv, a.group = (int)(p->H / p->Hk);
   a.scale = p->scale;
-  a.groups = (a.Dv + 15) / 16;
+  a.blocks = (int)blocks_of(p);
+  a.groups = 2 * a.blocks;
   const Sizes s = sizes_of(p);
   char* w = (char*)workspace;
   a.vecs = (float*)w, w += s.vecs;
-  if (!backward) {
-    a.tris = (__bf16*)w;
-  } else {
-    a.keys = (__bf16*)w, w += s.keys;
-    a.tris = (__bf16*)w, w += s.tris;
-    a.dstates = (float*)w, w += s.dstates;
-    a.drs = (float*)w;
+  a.tris = (__bf16*)w;
+  if (backward) {
+    w += s.back_tris;
+    a.ys = (float*)w, w += s.ys;
+    a.zs = (float*)w, w += s.zs;
+    a.dstates = (__bf16*)w, w += s.states;
+    a.drs = (__bf16*)w;
   }
+  a.states = (__bf16*)saved;
+  a.us = saved ? (__bf16*)((char*)saved + s.states) : nullptr;
   return a;
 }
 
@@ -1205,8 +1407,6 @@ int by_blocks(int64_t Dk, F f) {
   }
 }
 
-// Wavefronts of one workgroup of chain_back(), each with 16 columns.
-constexpr int kBackWaves = 4;
 dim3 chain_grid(const Args& a, int waves) {
   return dim3((unsigned)a.sequences, a.H, (a.groups + waves - 1) / waves);
 }
@@ -1223,18 +1423,19 @@ using namespace kd::delta;
 extern "C" size_t kdelta_scan_workspace_bytes(const kdelta_problem* p) {
   if (check(p)) return 0;
   const Sizes s = sizes_of(p);
-  return s.vecs + s.inv;
+  return s.vecs + s.tris;
 }
 
 extern "C" size_t kdelta_scan_bwd_workspace_bytes(const kdelta_problem* p) {
   if (check(p)) return 0;
   const Sizes s = sizes_of(p);
-  return s.vecs + s.keys + s.tris + s.dstates + s.drs;
+  return s.vecs + s.back_tris + s.ys + s.zs + s.states + s.rows;
 }
 
 extern "C" size_t kdelta_scan_saved_floats(const kdelta_problem* p) {
   if (check(p)) return 0;
-  return (size_t)tiles_of(p) * p->H * ((p->Dv + 15) / 16) * (2 * ((p->Dk + 31) / 32) + 4) * 256;
+  const Sizes s = sizes_of(p);
+  return (s.states + s.rows) / 4;
 }
 
 extern "C" int kdelta_scan_fwd(const kdelta_problem* p, void* o, const int64_t* o_strides, float* final, float* saved,
@@ -1249,11 +1450,9 @@ extern "C" int kdelta_scan_fwd(const kdelta_problem* p, void* o, const int64_t* 
     return fail(KDECAY_EWORKSPACE, "scan workspace of %zu bytes missing, small or not 16-byte aligned",
                 kdelta_scan_workspace_bytes(p));
   if ((uintptr_t)saved & 15) return fail(KDECAY_ELAYOUT, "saved is not 16-byte aligned");
-  Args a = args_of(p, workspace, false);
+  Args a = args_of(p, workspace, saved, false);
   a.o = o, a.final = final;
   if (rows) a.ob = o_strides[0], a.oh = o_strides[1], a.on = o_strides[2];
-  a.states = saved;
-  a.us = saved ? saved + (size_t)a.tiles * a.H * a.groups * 2 * ((a.Dk + 31) / 32) * 256 : nullptr;
   const hipStream_t s = (hipStream_t)stream;
   return by_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -1295,9 +1494,7 @@ extern "C" int kdelta_scan_bwd(const kdelta_problem* p, const void* d_o, const i
     return fail(KDECAY_EWORKSPACE, "backward workspace of %zu bytes missing, small or not 16-byte aligned",
                 kdelta_scan_bwd_workspace_bytes(p));
   if ((uintptr_t)saved & 15) return fail(KDECAY_ELAYOUT, "saved is not 16-byte aligned");
-  Args a = args_of(p, workspace, true);
-  a.states = const_cast<float*>(saved);
-  a.us = a.states + (size_t)a.tiles * a.H * a.groups * 2 * ((a.Dk + 31) / 32) * 256;
+  Args a = args_of(p, workspace, saved, true);
   a.d_o = d_o, a.d_final = d_final, a.d_init = d_init, a.dq = dq, a.dk = dk, a.dv = dv, a.dg = dg, a.dbeta = dbeta;
   if (rows) {
     a.dob = do_strides[0], a.doh = do_strides[1], a.don = do_strides[2];
@@ -1314,10 +1511,13 @@ extern "C" int kdelta_scan_bwd(const kdelta_problem* p, const void* d_o, const i
         prep<T, KB, true><<<dim3((unsigned)a.tiles, a.H), 256, 0, s>>>(a);
         if (const int rc = hip_check("kdelta prep launch")) return rc;
       }
-      chain_back<T, KB><<<chain_grid(a, kBackWaves), 64 * kBackWaves, 0, s>>>(a);
+      chain_back<T, KB><<<chain_grid(a, 4), 512, 0, s>>>(a);
       if (const int rc = hip_check("kdelta chain_back launch")) return rc;
       if (!rows) return 0;
-      grads<T, KB><<<dim3((unsigned)a.tiles, a.Hk), 256, 0, s>>>(a);
+      if (a.group > 1)
+        grads<T, KB, true><<<dim3((unsigned)a.tiles, a.Hk), 256, 0, s>>>(a);
+      else
+        grads<T, KB, false><<<dim3((unsigned)a.tiles, a.Hk), 256, 0, s>>>(a);
       return hip_check("kdelta grads launch");
     });
   });

@@ -159,6 +159,25 @@ __device__ __forceinline__ void settle(V (&x)[N]) {
   settle(x[0]);
 }
 
+typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes per lane from global memory to LDS, at `to` + 16 lane.  In assembly, because the compiler
+// takes the LDS that its own form of it writes for any LDS that is read later, and
+// waits for rows that are still to come before it reads those that are there; who
+// calls this waits itself (lds_copies_done, then a barrier).
+__device__ __forceinline__ void copy_to_lds(const void* from, const void* to) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LdsPtr)(void*)to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Eight bytes per lane, transposed among each 16 lanes: these read four rows of 16 16-bit values (lane j
+// the four at row j / 4, columns 4 (j % 4)..), and lane j gets column j's four.
+__device__ __forceinline__ u32x2 read_transposed(const void* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(LdsPtr)(void*)p));
+}
+
 // The wavefront's number in its workgroup, known to the compiler to be one for all its
 // lanes: branches on it are scalar, and barriers behind them are reached by whole wavefronts.
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
