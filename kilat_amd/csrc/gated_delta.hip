@@ -978,7 +978,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
 // those over the chunk's tokens, whose factors dO_i.u_j and dR_i.u_j are computed
 // both ways round, so that either is an operand as it stands.
 template <typename T, int KB, bool GROUPED>
-__global__ __launch_bounds__(256) void grads(Args a) {
+__global__ __launch_bounds__(256, KB <= 2 ? 2 : 1) void grads(Args a) {
   constexpr int NI = kInputTerms<T>;
   constexpr int SP = NX * 32 * 32 * KB, UP = NX * 32 * C, kKt = 4 * KB * NI * kFrag;
   constexpr int kPlanes = 2 * SP + 2 * UP + 4 * NI * kFrag;
@@ -1058,13 +1058,14 @@ __global__ __launch_bounds__(256) void grads(Args a) {
         hq[dt] = product<2>(s, o, hq[dt]);
         rho[dt] = product<2>(s, r, rho[dt]);
         kw[dt] = product<2>(ds, u, kw[dt]);
-        if (dt % 4 == w) {
+      }
+      settle(hq), settle(rho), settle(kw);
+      for (int dt = w; dt < 2 * KB; dt += 4) {  // <S, dS>: every fourth tile
+        const Terms<NX> s = load_plane<KB>(Sp, dt, lane), ds = load_plane<KB>(dSp, dt, lane);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            ss = fmaf(((float)s.t[2][i] + (float)s.t[1][i]) + (float)s.t[0][i],
-                      ((float)ds.t[2][i] + (float)ds.t[1][i]) + (float)ds.t[0][i], ss);
-        }
-        settle(hq[dt]), settle(rho[dt]), settle(kw[dt]);
+        for (int i = 0; i < 8; ++i)
+          ss = fmaf(((float)s.t[2][i] + (float)s.t[1][i]) + (float)s.t[0][i],
+                    ((float)ds.t[2][i] + (float)ds.t[1][i]) + (float)ds.t[0][i], ss);
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -1072,12 +1073,14 @@ __global__ __launch_bounds__(256) void grads(Args a) {
           const Terms<NX> uj = load_plane<2>(Up, x, lane);
           E1[x] = product<2>(uj, o, E1[x]);
           E2[x] = product<2>(uj, r, E2[x]);
-          settle(E1[x]), settle(E2[x]);
+          asm volatile("" : "+v"(E1[x]));
+          settle(E2[x]);
         }
         if (x >= w) {
           F1[x] = product<2>(load_terms<NI>(Of + x * NI * kFrag, lane), u, F1[x]);
           F2[x] = product<2>(load_plane<2>(Rp, x, lane), u, F2[x]);
-          settle(F1[x]), settle(F2[x]);
+          asm volatile("" : "+v"(F1[x]));
+          settle(F2[x]);
         }
       }
     }
@@ -1136,19 +1139,22 @@ __global__ __launch_bounds__(256) void grads(Args a) {
       const bool lo = kb <= w / 2, hi = kb >= w / 2;
       const Terms<NX> e1 = split<NX>(E1[2 * kb], E1[2 * kb + 1]), e2 = split<NX>(E2[2 * kb], E2[2 * kb + 1]);
       const Terms<NX> f1 = split<NX>(F1[2 * kb], F1[2 * kb + 1]), f2 = split<NX>(F2[2 * kb], F2[2 * kb + 1]);
+      if (lo) {
 #pragma unroll
-      for (int dt = 0; dt < 2 * KB; ++dt) {
-        const Terms<NI> kT = load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane);
-        if (lo) {
+        for (int dt = 0; dt < 2 * KB; ++dt) {
+          const Terms<NI> kT = load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane);
           hq[dt] = product<2>(kT, e1, hq[dt]);
           rho[dt] = product<2>(kT, e2, rho[dt]);
-          settle(hq[dt]), settle(rho[dt]);
         }
-        if (hi) {
+        settle(hq), settle(rho);
+      }
+      if (hi) {
+#pragma unroll
+        for (int dt = 0; dt < 2 * KB; ++dt) {
           kw[dt] = product<2>(load_terms<NI>(Qt + (dt * 2 + kb) * NI * kFrag, lane), f1, kw[dt]);
-          kw[dt] = product<2>(kT, f2, kw[dt]);
-          settle(kw[dt]);
+          kw[dt] = product<2>(load_terms<NI>(Kt + (dt * 2 + kb) * NI * kFrag, lane), f2, kw[dt]);
         }
+        settle(kw);
       }
     }
     T* dqrow = (T*)a.dq + bt * a.dqb + hk * a.dqh + (row0 + t) * a.dqn;
