@@ -57,6 +57,11 @@ struct Args {
   void* o;
   int64_t ob, oh, on;
   float* final;
+  // A sequence in `segs` pieces (1: whole): per sequence, head and piece, the state that
+  // a piece leaves of zero, how it carries a state over (planes, by its columns), and its first state
+  int segs;
+  float *seg_n, *seg_s;  // [sequences][H][segs][groups][2 KB][64][4]
+  __bf16* seg_m;         // [sequences][H][segs][KB][NX][32][32 KB]
   // backward
   const void* d_o;
   int64_t dob, doh, don;
@@ -461,12 +466,16 @@ __global__ __launch_bounds__(256) void prep(Args a) {
   }
 }
 
+// What a pass of chain() leaves: o (and the last state); what the backward reads as well; or, of a
+// piece of a sequence, how it carries states over.
+enum Mode { PLAIN, SAVE, TRANS };
+
 // --------------------------------------------------------------------------
 // chain: the chunks of one sequence and head, 16 columns of the state per wavefront
 // --------------------------------------------------------------------------
 // A chunk token by token, for the chunks that hold a value that is not finite: a
 // product with the zeros of T and P would carry it to earlier tokens.
-template <typename T, int KB, bool SAVE>
+template <typename T, int KB, int MODE>
 __device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, int64_t row0, int n, int h, int col,
                                             int64_t tile, f32x4 (&S)[2 * KB]) {
   const int hk = h / a.group, lane = threadIdx.x & 63, g = lane >> 4;
@@ -503,10 +512,11 @@ __device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, 
         }
       }
     }
+    if (MODE == TRANS) continue;
     o = group_sum(o);
     if (g == 0 && col < a.Dv) {
       ((T*)a.o)[rows.batch * a.ob + h * a.oh + (row0 + t) * a.on + col] = (T)(a.scale * o);
-      if (SAVE) {
+      if (MODE == SAVE) {
         const float y[8] = {u};
         const Terms<NX> e = split<NX>(y);
 #pragma unroll
@@ -526,36 +536,54 @@ __device__ __forceinline__ void chunk_by_token(const Args& a, const Rows& rows, 
 //   first part   chain: splits S, K S     feeders: T, V and K' of this chunk to LDS
 //   second part  chain: R, U, S           feeders: fetch the next chunk, P U of the one before,
 //                                         q S of this one, K of the next to LDS
-template <typename T, int KB, int NW, bool SAVE>
+template <typename T, int KB, int NW, int MODE>
 __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   constexpr int NI = kInputTerms<T>, NO = kOutTerms<T>, ORD = kOutOrder<T>;
   __shared__ __bf16 Kf[4 * KB * NI * kFrag], Kt[4 * KB * NI * kFrag], Tf[kTri * NX * kFrag];
   __shared__ float Vf[NW * 4 * 256];
   constexpr int kLds = (8 * KB * NI + kTri * NX + NW * KB * NO) * 1024 + NW * 4096 + 2 * V_CHAIN * C * 4 + 64;
   constexpr int UB = kLds + 2 * NW * 2 * NO * 1024 <= 160 * 1024 ? 2 : 1;  // buffers of U's terms
-  __shared__ __bf16 Sf[NW * KB * NO * kFrag], Uf[UB][NW * 2 * NO * kFrag];
+  __shared__ __bf16 Sf[MODE == TRANS ? 1 : NW * KB * NO * kFrag], Uf[UB][MODE == TRANS ? 1 : NW * 2 * NO * kFrag];
   __shared__ float vecs[2][V_CHAIN * C];
   __shared__ int by_token[2][NW];
-  const int64_t seq = blockIdx.x;
+  // (the last piece of a sequence carries nothing over)
+  const int pieces = MODE == TRANS ? a.segs - 1 : a.segs;
+  const int64_t seq = blockIdx.x / pieces;
+  const int seg = blockIdx.x % pieces;
   const int h = blockIdx.y, hk = h / a.group;
   const int wave = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const Rows rows = rows_of(a.cu, seq, a.N);
-  const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), nch = (rows.n + C - 1) / C;
-  const int col0 = blockIdx.z * 16 * NW;
+  const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), all = (rows.n + C - 1) / C;
+  const int64_t each = a.segs == 1 ? all : ((unsigned)all + a.segs - 1) / (unsigned)a.segs;  // chunks of a piece
+  const int64_t first = seg * each < all ? seg * each : all, nch = first + each < all ? first + each : all;
+  // TRANS: workgroups of v's columns, from zero (the first piece: from the state before it), then of the
+  // identity's with no v, which the first piece needs none of.
+  const int zv = (a.groups + NW - 1) / NW;
+  const bool unit = MODE == TRANS && (int)blockIdx.z >= zv;
+  if (unit && seg == 0) return;
+  const int col0 = ((int)blockIdx.z - (unit ? zv : 0)) * 16 * NW, width = unit ? 0 : a.Dv;  // columns of v there are
+  const int64_t piece = (seq * a.H + h) * a.segs + seg;
   if (wave < NW) {
     const int col = col0 + 16 * wave + m;
     const int cg = (col0 >> 4) + wave;
-    const bool in = col < a.Dv, any = cg < a.groups;
+    const bool in = col < width, any = cg < (unit ? 2 * KB : a.groups);
     f32x4 S[2 * KB];
 #pragma unroll
-    for (int dt = 0; dt < 2 * KB; ++dt)
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      if (MODE != TRANS && seg > 0) {
+        S[dt] = *reinterpret_cast<const f32x4*>(a.seg_s + ((piece * a.groups + (any ? cg : 0)) * 2 * KB + dt) * 256 + lane * 4);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = channel(dt, 4 * g + i);
-        S[dt][i] = a.init && in && d < a.Dk ? a.init[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          const int d = channel(dt, 4 * g + i);
+          S[dt][i] = unit ? (d == col ? 1.f : 0.f)
+                     : a.init && seg == 0 && in && d < a.Dk ? a.init[((seq * a.H + h) * a.Dk + d) * a.Dv + col]
+                                                            : 0.f;
+        }
       }
-    if (nch) lds_barrier();
-    for (int64_t c = 0; c < nch; ++c) {
+    }
+    if (first < nch) lds_barrier();
+    for (int64_t c = first; c < nch; ++c) {
       const int64_t tile = tile0 + c;
       const float* vec = vecs[c & 1];
       f32x4 X[4];
@@ -564,11 +592,13 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+          if (MODE != TRANS) {
 #pragma unroll
-          for (int j = 0; j < NO; ++j)
-            *reinterpret_cast<bf16x8*>(Sf + ((wave * KB + kb) * NO + j) * kFrag + lane * 8) = s[kb].t[j];
+            for (int j = 0; j < NO; ++j)
+              *reinterpret_cast<bf16x8*>(Sf + ((wave * KB + kb) * NO + j) * kFrag + lane * 8) = s[kb].t[j];
+          }
         }
-        if (SAVE) keep_state<KB>(a.states + planes_of<KB>(a, tile, h, cg >> 1), cg, m, g, s);
+        if (MODE == SAVE) keep_state<KB>(a.states + planes_of<KB>(a, tile, h, cg >> 1), cg, m, g, s);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) X[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -613,17 +643,17 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
         const bool slow = __any(!(fabsf(odd) <= 3.402823466e38f));  // something is not finite
         if (lane == 0) by_token[c & 1][wave] = slow;
         if (slow) {
-          chunk_by_token<T, KB, SAVE>(a, rows, rows.first + c * C, rows.n - c * C < C ? (int)(rows.n - c * C) : C, h, col,
-                                      tile, S);
+          chunk_by_token<T, KB, MODE>(a, rows, rows.first + c * C, rows.n - c * C < C ? (int)(rows.n - c * C) : C, h,
+                                      unit ? a.Dv : col, tile, S);  // (column Dv: v is 0)
         } else {
-          if (SAVE) {
-            const Terms<NX> u[2] = {split<NX>(U[0], U[1]), split<NX>(U[2], U[3])};
-            keep_rows(a.us + planes_of<2>(a, tile, h, cg >> 1), cg, m, g, u);
-          }
+          if (MODE != TRANS) {
+            const Terms<MODE == SAVE ? NX : NO> u[2] = {split<MODE == SAVE ? NX : NO>(U[0], U[1]), split<MODE == SAVE ? NX : NO>(U[2], U[3])};
+            if constexpr (MODE == SAVE) keep_rows(a.us + planes_of<2>(a, tile, h, cg >> 1), cg, m, g, u);
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const Terms<NO> u = split<NO>(U[2 * kb], U[2 * kb + 1]);
-            store_terms<NO>(Uf[c & (UB - 1)] + (wave * 2 + kb) * NO * kFrag, lane, u);
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int j = 0; j < NO; ++j)
+                *reinterpret_cast<bf16x8*>(Uf[c & (UB - 1)] + ((wave * 2 + kb) * NO + j) * kFrag + lane * 8) = u[kb].t[j];
           }
           const float whole = vec[V_SINCE * C + C - 1];
 #pragma unroll
@@ -643,7 +673,19 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
       }
       lds_barrier();
     }
-    if (a.final) {
+    if (MODE == TRANS) {
+      if (!any) return;
+      if (unit) {
+        Terms<NX> s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+        keep_state<KB>(a.seg_m + (piece * KB + (cg >> 1)) * (int64_t)(NX * 32 * 32 * KB), cg, m, g, s);
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < 2 * KB; ++dt)
+          *reinterpret_cast<f32x4*>(a.seg_n + ((piece * a.groups + cg) * 2 * KB + dt) * 256 + lane * 4) = S[dt];
+      }
+    } else if (a.final && seg + 1 == a.segs) {
 #pragma unroll
       for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
@@ -654,7 +696,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     }
     return;
   }
-  if (!nch) return;
+  if (first >= nch) return;
   // A feeder: tokens 16w + m of each chunk.
   const int w = wave - NW, t = 16 * w + m, ft = threadIdx.x - 64 * NW;
   const T* kbase = (const T*)a.k + rows.batch * a.kb + hk * a.kh + rows.first * a.kn;
@@ -663,29 +705,30 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   T* obase = (T*)a.o + rows.batch * a.ob + h * a.oh + rows.first * a.on;
   constexpr int VB = (NW + 1) / 2;             // 32-column blocks of V
   constexpr int TP = (kTri * NX + 3) / 4;      // planes of T per feeder: w, w + 4, ...
-  const T *kp = kbase + t * a.kn + 8 * g, *qp = qbase + t * a.qn + 8 * g, *vp = vbase + t * a.vn + col0 + 8 * g;
-  const __bf16* ip = tri_tiles<T, false>(a, tile0, h) + w * kFrag + lane * 8;
-  const __bf16* pp = tri_tiles<T, false>(a, tile0, h) + (kTri * NX + tri_lower(w, 0) * NO) * kFrag + lane * 8;
-  const float* ep = vec_of(a, tile0, h) + (ft % (V_CHAIN * C / 4)) * 4;
+  const int64_t t0 = first * C + t;
+  const T *kp = kbase + t0 * a.kn + 8 * g, *qp = qbase + t0 * a.qn + 8 * g, *vp = vbase + t0 * a.vn + col0 + 8 * g;
+  const __bf16* ip = tri_tiles<T, false>(a, tile0 + first, h) + w * kFrag + lane * 8;
+  const __bf16* pp = tri_tiles<T, false>(a, tile0 + first, h) + (kTri * NX + tri_lower(w, 0) * NO) * kFrag + lane * 8;
+  const float* ep = vec_of(a, tile0 + first, h) + (ft % (V_CHAIN * C / 4)) * 4;
   Raw8<T> kr[KB], qr[KB], vr[VB];
   bf16x8 tr[TP];
   Terms<NO> pr[2] = {};
   f32x4 er;
-  int left = rows.n < t ? 0 : rows.n - t < 0x7fffffff ? (int)(rows.n - t) : 0x7fffffff;  // rows from this lane's on
+  int left = rows.n < t0 ? 0 : rows.n - t0 < 0x7fffffff ? (int)(rows.n - t0) : 0x7fffffff;  // rows from this lane's on
   const auto fetch = [&]() {  // the next chunk's
-    const int dk = left > 0 ? a.Dk - 8 * g : 0, dv = left > 0 ? a.Dv - col0 - 8 * g : 0;
+    const int dk = left > 0 ? a.Dk - 8 * g : 0, dv = left > 0 ? width - col0 - 8 * g : 0;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       kr[kb] = *reinterpret_cast<const Raw8<T>*>(32 * kb < dk ? kp + 32 * kb : kbase);
-      qr[kb] = *reinterpret_cast<const Raw8<T>*>(32 * kb < dk ? qp + 32 * kb : qbase);
+      if (MODE != TRANS) qr[kb] = *reinterpret_cast<const Raw8<T>*>(32 * kb < dk ? qp + 32 * kb : qbase);
     }
 #pragma unroll
     for (int b = 0; b < VB; ++b) vr[b] = *reinterpret_cast<const Raw8<T>*>(32 * b < dv ? vp + 32 * b : vbase);
 #pragma unroll
     for (int x = 0; x < TP; ++x)
       if (4 * x + 4 <= kTri * NX || w + 4 * x < kTri * NX) tr[x] = *reinterpret_cast<const bf16x8*>(ip + 4 * x * kFrag);
-    pr[0] = load_terms<NO>(pp, 0);
-    if (w >= 2) pr[1] = load_terms<NO>(pp + NO * kFrag, 0);
+    if (MODE != TRANS) pr[0] = load_terms<NO>(pp, 0);
+    if (MODE != TRANS && w >= 2) pr[1] = load_terms<NO>(pp + NO * kFrag, 0);
     er = *reinterpret_cast<const f32x4*>(ep);
     kp += C * a.kn, qp += C * a.qn, vp += C * a.vn;
     ip += a.H * (int64_t)kTriSize<T, false>, pp += a.H * (int64_t)kTriSize<T, false>, ep += a.H * (int64_t)(V_COUNT * C);
@@ -704,7 +747,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   const bf16x8 ksel[2] = {selector(channel(0, m), g), selector(channel(1, m), g)};
   const bf16x8 vsel[2] = {selector(m, g), selector(16 + m, g)};
   fetch();
-  put_keys(0);
+  put_keys(first);
   lds_barrier();
   Terms<NO> p[2];  // P of the last chunk: lane m = token i, inner indices j
   f32x4 O[NW];     // scale e^G S' q of it
@@ -725,7 +768,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     for (int x = 0; x < NW; ++x)
       if (c * C + t < rows.n && col0 + 16 * x + 4 * g < a.Dv && !by_token[c & 1][x]) store4(row + 16 * x, O[x] + y[x]);
   };
-  for (int64_t c = 0; c < nch; ++c) {
+  for (int64_t c = first; c < nch; ++c) {
     const float* vec = vecs[c & 1];
 #pragma unroll
     for (int x = 0; x < TP; ++x)
@@ -744,7 +787,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
         *reinterpret_cast<u32x2*>(Kt + (((2 * kb + x / NI) * 2 + (w >> 1)) * NI + x % NI) * kFrag + lane * 8 + 4 * (w & 1)) = r;
       }
     }
-    const int dv = left > 0 ? a.Dv - col0 - 8 * g : 0;
+    const int dv = left > 0 ? width - col0 - 8 * g : 0;
 #pragma unroll
     for (int b = 0; b < VB; ++b) {
       const Terms<NI> v = terms_of<T>(vr[b], dv - 32 * b);
@@ -761,33 +804,93 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
         if (2 * b + x < NW) *reinterpret_cast<f32x4*>(Vf + ((2 * b + x) * 4 + w) * 256 + lane * 4) = z[x];
     }
     Terms<NI> q[KB];
-    const int dk = left > 0 ? a.Dk - 8 * g : 0;
+    if (MODE != TRANS) {
+      const int dk = left > 0 ? a.Dk - 8 * g : 0;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) q[kb] = terms_of<T>(qr[kb], dk - 32 * kb);
+      for (int kb = 0; kb < KB; ++kb) q[kb] = terms_of<T>(qr[kb], dk - 32 * kb);
+    }
     left -= C;
-    if (UB == 1 && c) write_out(c - 1, p, O);
+    if (MODE != TRANS && UB == 1 && c > first) write_out(c - 1, p, O);
     const Terms<NO> p1[2] = {pr[0], pr[1]};
     lds_barrier();
     if (c + 1 < nch) fetch();
-    if (UB == 2 && c) write_out(c - 1, p, O);
-    p[0] = p1[0], p[1] = p1[1];
-    const float since = a.scale * vec[V_SINCE * C + t];
+    if (MODE != TRANS) {
+      if (UB == 2 && c > first) write_out(c - 1, p, O);
+      p[0] = p1[0], p[1] = p1[1];
+      const float since = a.scale * vec[V_SINCE * C + t];
 #pragma unroll
-    for (int x = 0; x < NW; ++x) O[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < NW; ++x) O[x] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      Terms<NO> y[NW];
+      for (int kb = 0; kb < KB; ++kb) {
+        Terms<NO> y[NW];
 #pragma unroll
-      for (int x = 0; x < NW; ++x) y[x] = load_terms<NO>(Sf + (x * KB + kb) * NO * kFrag, lane);
-      products<ORD>(y, q[kb], O);
+        for (int x = 0; x < NW; ++x) y[x] = load_terms<NO>(Sf + (x * KB + kb) * NO * kFrag, lane);
+        products<ORD>(y, q[kb], O);
+      }
+      settle(O);
+#pragma unroll
+      for (int x = 0; x < NW; ++x) O[x] *= since;
     }
-    settle(O);
-#pragma unroll
-    for (int x = 0; x < NW; ++x) O[x] *= since;
     if (c + 1 < nch) put_keys(c + 1);
     lds_barrier();
   }
-  write_out(nch - 1, p, O);
+  if (MODE != TRANS) write_out(nch - 1, p, O);
+}
+
+// The first state of every piece, one piece after another: S <- M S + N.  A wavefront has 16 columns; M comes
+// through LDS, 32 of its columns at a time, the next ones while these are multiplied.
+template <int KB>
+__global__ __launch_bounds__(256) void join(Args a) {
+  constexpr int kBlock = NX * 32 * 32 * KB;
+  __shared__ __align__(16) __bf16 Ms[2][kBlock];
+  const int64_t seq = blockIdx.x;
+  const int h = blockIdx.y;
+  const int w = wave_index(), lane = threadIdx.x & 63, j = lane & 15, row = 8 * (lane >> 4) + (j >> 2);
+  const int cg = blockIdx.z * 4 + w, cgr = cg < a.groups ? cg : 0;
+  const int64_t piece0 = (seq * a.H + h) * a.segs;
+  const auto at = [&](int seg) { return (((piece0 + seg) * a.groups + cgr) * 2 * KB) * 256 + lane * 4; };
+  const int steps = (a.segs - 2) * KB;  // pieces 1 .. segs - 2
+  const auto copy = [&](int i) {
+    const __bf16* from = a.seg_m + ((piece0 + 1) * KB + i) * (int64_t)kBlock + lane * 8;
+    for (int x = w; x < kBlock / kFrag; x += 4) copy_to_lds(from + x * kFrag, Ms[i & 1] + x * kFrag);
+  };
+  if (steps) copy(0);
+  f32x4 S[2 * KB];
+#pragma unroll
+  for (int dt = 0; dt < 2 * KB; ++dt) S[dt] = *reinterpret_cast<const f32x4*>(a.seg_n + at(0) + dt * 256);
+  for (int seg = 1; seg < a.segs; ++seg) {
+    if (cg < a.groups) {
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt) *reinterpret_cast<f32x4*>(a.seg_s + at(seg) + dt * 256) = S[dt];
+    }
+    if (seg + 1 == a.segs) break;
+    Terms<NX> s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+#pragma unroll
+    for (int dt = 0; dt < 2 * KB; ++dt) S[dt] = *reinterpret_cast<const f32x4*>(a.seg_n + at(seg) + dt * 256);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int i = (seg - 1) * KB + kb;
+      lds_copies_done();
+      __syncthreads();
+      if (i + 1 < steps) copy(i + 1);
+#pragma unroll
+      for (int dt = 0; dt < 2 * KB; ++dt) {
+        // M's rows in the order of a state's: each lane reads the four channels that come next in it
+        Terms<NX> x;
+#pragma unroll
+        for (int n = 0; n < NX; ++n) {
+          const __bf16* p = Ms[i & 1] + n * 32 * 32 * KB;
+          const u32x2 y = read_transposed(p + plane_at<KB>(row, channel(dt, 4 * (j & 3))));
+          const u32x2 z = read_transposed(p + plane_at<KB>(row + 4, channel(dt, 4 * (j & 3))));
+          x.t[n] = __builtin_bit_cast(bf16x8, make_uint4(y.x, y.y, z.x, z.y));
+        }
+        S[dt] = product<2>(x, s[kb], S[dt]);
+      }
+      settle(S);
+    }
+  }
 }
 
 // --------------------------------------------------------------------------
@@ -1323,8 +1426,39 @@ int input_terms(int dtype) { return dtype == KDECAY_BF16 ? 1 : dtype == KDECAY_F
 
 int64_t blocks_of(const kdelta_problem* p) { return (p->Dv + 31) / 32; }
 
+// Wavefronts of a workgroup of chain(): four, and fewer where three terms of wide keys leave no room in
+// LDS for as many.
+constexpr int chain_waves(int element_size, int KB) { return element_size == 2 || KB <= 2 ? 4 : KB == 3 ? 2 : 1; }
+
+// Pieces that a sequence is cut into. A workgroup of chain() takes 3 to 5 us per chunk in 16-bit types (about 9
+// in float32) and fills a CU, so few streams leave most of the card idle; pieces cost a
+// pass over all of them but the last first (about 0.65 of that per chunk, and as many more
+// workgroups as a state has columns of its own), a join of 1 to 3 us per piece and two launches.
+// Measured (us, whole / pieces): B=1 H=16 N=65536 D=128 bf16 4212 / 1461 with 8, 1896 with 4, 1653 with 16;
+// B=8 H=6 N=1024 D=64 64 / 52 with 4, 69 with 6; B=4 H=16 N=2047 D=80 fp16 202 / 179
+// with 2, 221 with 4; B=2 H=6 N=1024 D=64 float32 (with the backward) 266 / 163 with 8.  (A packed batch: by the
+// mean length.)
+int pieces_of(const kdelta_problem* p) {
+  constexpr double kCus = 256, kPass = 0.65, kFixed = 4;
+  if (!p->sequences) return 1;
+  const int64_t KB = (p->Dk + 31) / 32, NW = chain_waves(p->dtype == KDECAY_F32 ? 4 : 2, (int)KB);
+  const int64_t zv = (2 * ((p->Dv + 31) / 32) + NW - 1) / NW, zk = (2 * KB + NW - 1) / NW;
+  const int64_t chunks = (p->N / (p->cu_seqlens ? p->sequences : 1) + C - 1) / C;
+  const double streams = (double)p->sequences * p->H, join = 0.75 * KB;
+  const double step = p->dtype == KDECAY_F32 ? 9 : (KB <= 2 ? 3 : 4) + (p->dtype == KDECAY_F16 ? 1 : 0);
+  const auto rounds = [](double n) { return ceil(n / kCus); };
+  int best = 1;
+  double least = 0.9 * rounds(streams * zv) * chunks * step;
+  for (int n = 2; n <= 16 && 2 * n <= chunks; ++n) {
+    const double each = (double)((chunks + n - 1) / n);
+    const double cost = each * step * (rounds(streams * zv * n) + kPass * rounds(streams * (n - 1) * (zv + zk))) + join * n + kFixed;
+    if (cost < least) least = cost, best = n;
+  }
+  return best;
+}
+
 struct Sizes {  // bytes
-  size_t vecs, tris, back_tris, ys, zs, states, rows;
+  size_t vecs, tris, back_tris, ys, zs, states, rows, seg_n, seg_m;
 };
 
 Sizes sizes_of(const kdelta_problem* p) {
@@ -1337,6 +1471,9 @@ Sizes sizes_of(const kdelta_problem* p) {
   s.zs = up256(heads * 2 * blocks * 2 * KB * 256 * 4);
   s.states = up256(heads * blocks * NX * 32 * 32 * KB * 2);
   s.rows = up256(heads * blocks * NX * 32 * C * 2);
+  const size_t segs = pieces_of(p), pieces = segs > 1 ? (size_t)p->sequences * p->H * segs : 0;
+  s.seg_n = up256(pieces * 2 * blocks * 2 * KB * 256 * 4);
+  s.seg_m = up256(pieces * KB * NX * 32 * 32 * KB * 2);
   return s;
 }
 
@@ -1381,7 +1518,14 @@ Args args_of(const kdelta_problem* p, void* workspace, const float* saved, bool 
   char* w = (char*)workspace;
   a.vecs = (float*)w, w += s.vecs;
   a.tris = (__bf16*)w;
-  if (backward) {
+  a.segs = 1;
+  if (!backward) {
+    w += s.tris;
+    a.segs = pieces_of(p);
+    a.seg_n = (float*)w, w += s.seg_n;
+    a.seg_s = (float*)w, w += s.seg_n;
+    a.seg_m = (__bf16*)w;
+  } else {
     w += s.back_tris;
     a.ys = (float*)w, w += s.ys;
     a.zs = (float*)w, w += s.zs;
@@ -1414,12 +1558,8 @@ int by_blocks(int64_t Dk, F f) {
 }
 
 dim3 chain_grid(const Args& a, int waves) {
-  return dim3((unsigned)a.sequences, a.H, (a.groups + waves - 1) / waves);
+  return dim3((unsigned)(a.sequences * a.segs), a.H, (a.groups + waves - 1) / waves);
 }
-// Of chain(): four, and fewer where three terms of wide keys leave no room in LDS for as many.
-template <typename T, int KB>
-constexpr int kChainWaves = sizeof(T) == 2 || KB <= 2 ? 4 : KB == 3 ? 2 : 1;
-
 }  // namespace delta
 }  // namespace kd
 
@@ -1429,7 +1569,7 @@ using namespace kd::delta;
 extern "C" size_t kdelta_scan_workspace_bytes(const kdelta_problem* p) {
   if (check(p)) return 0;
   const Sizes s = sizes_of(p);
-  return s.vecs + s.tris;
+  return s.vecs + s.tris + 2 * s.seg_n + s.seg_m;
 }
 
 extern "C" size_t kdelta_scan_bwd_workspace_bytes(const kdelta_problem* p) {
@@ -1468,11 +1608,19 @@ extern "C" int kdelta_scan_fwd(const kdelta_problem* p, void* o, const int64_t* 
         prep<T, KB, false><<<dim3((unsigned)a.tiles, a.H), 256, 0, s>>>(a);
         if (const int rc = hip_check("kdelta prep launch")) return rc;
       }
-      constexpr int NW = kChainWaves<T, KB>;
+      constexpr int NW = chain_waves(sizeof(T), KB);
+      const dim3 grid = chain_grid(a, NW);
+      if (a.segs > 1) {
+        const dim3 pieces((unsigned)(a.sequences * (a.segs - 1)), a.H, grid.z + (2 * KB + NW - 1) / NW);
+        chain<T, KB, NW, TRANS><<<pieces, 64 * (NW + 4), 0, s>>>(a);
+        if (const int rc = hip_check("kdelta chain launch")) return rc;
+        join<KB><<<dim3((unsigned)a.sequences, a.H, (a.groups + 3) / 4), 256, 0, s>>>(a);
+        if (const int rc = hip_check("kdelta join launch")) return rc;
+      }
       if (saved)
-        chain<T, KB, NW, true><<<chain_grid(a, NW), 64 * (NW + 4), 0, s>>>(a);
+        chain<T, KB, NW, SAVE><<<grid, 64 * (NW + 4), 0, s>>>(a);
       else
-        chain<T, KB, NW, false><<<chain_grid(a, NW), 64 * (NW + 4), 0, s>>>(a);
+        chain<T, KB, NW, PLAIN><<<grid, 64 * (NW + 4), 0, s>>>(a);
       return hip_check("kdelta chain launch");
     });
   });
