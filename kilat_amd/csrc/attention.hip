@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
   const int64_t last = q0 + BQ < n ? q0 + BQ : n;
   const int steps = (int)((last + BK - 1) / BK), mine = (int)((q0 + 32 * w + 32 + BK - 1) / BK);  // of this wavefront's rows
 
-  const auto step = [&](int i, auto masked_of) {
+  const auto step = [&](int i, auto masked_of) __attribute__((always_inline)) {
     constexpr bool masked = decltype(masked_of)::value;
     const char* kl = reinterpret_cast<const char*>(kbuf[i & 1]);
     const char* vl = reinterpret_cast<const char*>(vbuf[i & 1]);

@@ -434,7 +434,7 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       }
       __syncthreads();
       const int64_t cg = (tile * a.H + h) * a.groups + (c0 >> 4);
-      const auto times_do = [&](const Terms<NX> (&x)[2], float* to, int64_t step) {
+      const auto times_do = [&](const Terms<NX> (&x)[2], float* to, int64_t step) __attribute__((always_inline)) {
         f32x4 y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -715,7 +715,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   Terms<NO> pr[2] = {};
   f32x4 er;
   int left = rows.n < t0 ? 0 : rows.n - t0 < 0x7fffffff ? (int)(rows.n - t0) : 0x7fffffff;  // rows from this lane's on
-  const auto fetch = [&]() {  // the next chunk's
+  const auto fetch = [&]() __attribute__((always_inline)) {  // the next chunk's
     const int dk = left > 0 ? a.Dk - 8 * g : 0, dv = left > 0 ? width - col0 - 8 * g : 0;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -734,7 +734,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     ip += a.H * (int64_t)kTriSize<T, false>, pp += a.H * (int64_t)kTriSize<T, false>, ep += a.H * (int64_t)(V_COUNT * C);
   };
   Terms<NI> kt[KB];
-  const auto put_keys = [&](int64_t c) {
+  const auto put_keys = [&](int64_t c) __attribute__((always_inline)) {
     const int dk = left > 0 ? a.Dk - 8 * g : 0;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -751,7 +751,7 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
   lds_barrier();
   Terms<NO> p[2];  // P of the last chunk: lane m = token i, inner indices j
   f32x4 O[NW];     // scale e^G S' q of it
-  const auto write_out = [&](int64_t c, const Terms<NO> (&p)[2], const f32x4 (&O)[NW]) {
+  const auto write_out = [&](int64_t c, const Terms<NO> (&p)[2], const f32x4 (&O)[NW]) __attribute__((always_inline)) {
     f32x4 y[NW];
 #pragma unroll
     for (int x = 0; x < NW; ++x) y[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -811,12 +811,17 @@ __global__ __launch_bounds__(64 * (NW + 4)) void chain(Args a) {
     }
     left -= C;
     if (MODE != TRANS && UB == 1 && c > first) write_out(c - 1, p, O);
-    const Terms<NO> p1[2] = {pr[0], pr[1]};
+    // The next chunk is fetched as early as registers allow: with one term per input, before P U, whose P
+    // then has to be another than the one that comes.
+    constexpr bool early = NI == 1;
+    Terms<NO> p1[2];
+    if (early) p1[0] = pr[0], p1[1] = pr[1];
     lds_barrier();
-    if (c + 1 < nch) fetch();
+    if ((early || MODE == TRANS) && c + 1 < nch) fetch();
     if (MODE != TRANS) {
       if (UB == 2 && c > first) write_out(c - 1, p, O);
-      p[0] = p1[0], p[1] = p1[1];
+      p[0] = early ? p1[0] : pr[0], p[1] = early ? p1[1] : pr[1];
+      if (!early && c + 1 < nch) fetch();
       const float since = a.scale * vec[V_SINCE * C + t];
 #pragma unroll
       for (int x = 0; x < NW; ++x) O[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -848,9 +853,9 @@ __global__ __launch_bounds__(256) void join(Args a) {
   const int w = wave_index(), lane = threadIdx.x & 63, j = lane & 15, row = 8 * (lane >> 4) + (j >> 2);
   const int cg = blockIdx.z * 4 + w, cgr = cg < a.groups ? cg : 0;
   const int64_t piece0 = (seq * a.H + h) * a.segs;
-  const auto at = [&](int seg) { return (((piece0 + seg) * a.groups + cgr) * 2 * KB) * 256 + lane * 4; };
+  const auto at = [&](int seg) __attribute__((always_inline)) { return (((piece0 + seg) * a.groups + cgr) * 2 * KB) * 256 + lane * 4; };
   const int steps = (a.segs - 2) * KB;  // pieces 1 .. segs - 2
-  const auto copy = [&](int i) {
+  const auto copy = [&](int i) __attribute__((always_inline)) {
     const __bf16* from = a.seg_m + ((piece0 + 1) * KB + i) * (int64_t)kBlock + lane * 8;
     for (int x = w; x < kBlock / kFrag; x += 4) copy_to_lds(from + x * kFrag, Ms[i & 1] + x * kFrag);
   };
@@ -930,7 +935,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
         const int d = channel(dt, 4 * g + i);
         S[dt][i] = a.d_final && in && d < a.Dk ? a.d_final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
       }
-    const auto fetch = [&](int64_t c) {
+    const auto fetch = [&](int64_t c) __attribute__((always_inline)) {
       const int64_t at = ((tile0 + c) * a.H + h) * a.groups + (any ? cg : 0);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) Y[mt] = *reinterpret_cast<const f32x4*>(a.ys + (at * 4 + mt) * 256 + lane * 4);
@@ -1027,8 +1032,8 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
   Raw8<T> kr[KB];
   bf16x8 tr[TP];
   f32x4 er;
-  const auto left_of = [&](int64_t c) { return c * C + t < rows.n ? a.Dk - 8 * g : 0; };
-  const auto fetch = [&](int64_t c) {
+  const auto left_of = [&](int64_t c) __attribute__((always_inline)) { return c * C + t < rows.n ? a.Dk - 8 * g : 0; };
+  const auto fetch = [&](int64_t c) __attribute__((always_inline)) {
     const int dk = left_of(c);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) kr[kb] = fetch8(kbase, (c * C + t) * a.kn + 32 * kb + 8 * g, dk - 32 * kb);
@@ -1039,7 +1044,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
     er = *reinterpret_cast<const f32x4*>(vec_of(a, tile0 + c, h) + (ft % (V_CHAIN * C / 4)) * 4);
   };
   Terms<NI> kt[KB];
-  const auto put_keys = [&](int64_t c) {
+  const auto put_keys = [&](int64_t c) __attribute__((always_inline)) {
     const int dk = left_of(c);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {

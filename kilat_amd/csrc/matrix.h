@@ -165,10 +165,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 // 16 bytes per lane from global memory to LDS, at `to` + 16 lane.  In assembly, because the compiler
 // takes the LDS that its own form of it writes for any LDS that is read later, and
 // waits for rows that are still to come before it reads those that are there; who
-// calls this waits itself (lds_copies_done, then a barrier).
+// calls this waits itself (lds_copies_done, then a barrier).  (M0 has no other use in these kernels.)
 __device__ __forceinline__ void copy_to_lds(const void* from, const void* to) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LdsPtr)(void*)to);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
 }
 __device__ __forceinline__ void lds_copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
