@@ -325,6 +325,8 @@ struct Stage {
     }
   }
   // Rows k0.. of n, into `to`; rows behind the last are copies of it.
+  // The next call's are G steps on.
+  template <int G>
   __device__ __forceinline__ void load(T* to, int64_t k0, int64_t n, int64_t stride, int w) {
     if (k0 + BK <= n) {
 #pragma unroll
@@ -339,7 +341,7 @@ struct Stage {
       }
     }
 #pragma unroll
-    for (int i = 0; i < NL; ++i) p[i] += BK * stride;
+    for (int i = 0; i < NL; ++i) p[i] += G * BK * stride;
   }
 };
 
@@ -350,11 +352,30 @@ __device__ __forceinline__ unsigned not_finite(unsigned x) {
   return (((x & 0x7fff7fffu) + top) >> 15 & 0x00010001u) * 0xffffu;
 }
 
-template <typename T, int KS, int VT>
-__global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
+// The tile that the `order`-th workgroup of a head takes in a packed batch of up to 64 sequences: the longest
+// sequence's first, each sequence's last tile first, so that what is left at the end is
+// short.  (-1: there are no more.)  A lane has a sequence.
+__device__ __forceinline__ int64_t longest_first(const Args& a, int64_t order, int lane) {
+  const Rows rows = lane < a.sequences ? rows_of(a.cu, lane, a.N) : Rows{0, 0, 0};
+  const int tiles = (int)((rows.n + BQ - 1) / BQ);
+  int before = 0;  // tiles of longer sequences
+  for (int s = 0; s < (int)a.sequences; ++s) {
+    const int other = __builtin_amdgcn_readlane(tiles, s);
+    before += other > tiles || (other == tiles && s < lane) ? other : 0;
+  }
+  const unsigned long long found = __ballot(order >= before && order < before + tiles);
+  if (!found) return -1;
+  const int64_t tile = rows.first / BQ + lane + (before + tiles - 1 - order);
+  const int at = __ffsll(found) - 1;
+  return __builtin_amdgcn_readlane((int)tile, at);  // (tiles are fewer than 2^31)
+}
+
+template <typename T, int KS, int VT, int G>
+__global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void forward16(Args a) {
   typedef typename Vec8<T>::type V8;
   constexpr int KC = 2 * KS, VC = 4 * VT;  // chunks of a row
-  __shared__ __align__(16) T kbuf[2][BK * KC * 8], vbuf[2][BK * VC * 8];
+  constexpr int kKeys = BK * KC * 8, kValues = BK * VC * 8;
+  __shared__ __align__(16) T lds[G * 2 * (kKeys + kValues)];
   // Workgroups go to the eight XCDs in turn.  With a multiple of eight heads each XCD has heads of
   // its own, so the keys that its workgroups read at the same time are the same; the tiles
   // with the most keys go first.
@@ -368,24 +389,29 @@ __global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
     tile = order % seqs * (int64_t)each + (each - 1 - order / seqs);
   }
   const int hk = h / a.group;
-  const int tid = threadIdx.x, w = wave_index(), lane = tid & 63, n32 = lane & 31, half = lane >> 5;
-  zero_outside<BQ>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, tid, kThreads);
+  const int tid = threadIdx.x, lane = tid & 63, n32 = lane & 31, half = lane >> 5;
+  const int part = G == 1 ? 0 : wave_index() / kWaves, w = wave_index() % kWaves;  // steps part, part + G, ...; rows 32w..
+  T *kbuf = lds + part * 2 * (kKeys + kValues), *vbuf = kbuf + 2 * kKeys;
+  zero_outside<BQ>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, tid, kThreads * G);
+  if (a.cu && a.sequences <= 64) {
+    tile = longest_first(a, order, lane);
+    if (tile < 0) return;
+  }
   const TileOf at = tile_of<BQ>(a.cu, a.sequences, tile, a.N);
   const int64_t q0 = at.index * BQ, n = at.rows.n;
   if (n <= q0) return;
   const T* kp = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + at.rows.first * a.kn;
   const T* vp = (const T*)a.v + at.rows.batch * a.vb + hk * a.vh + at.rows.first * a.vn;
   if (a.Dk < KS * 16 || a.Dv < VT * 32) {  // padding chunks are zero throughout
-    for (int i = tid; i < 2 * BK * KC; i += kThreads) reinterpret_cast<uint4*>(kbuf)[i] = make_uint4(0, 0, 0, 0);
-    for (int i = tid; i < 2 * BK * VC; i += kThreads) reinterpret_cast<uint4*>(vbuf)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < G * 2 * BK * (KC + VC); i += kThreads * G) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
   Stage<T, KC> sk;
   Stage<T, VC> sv;
-  sk.init(kp, a.kn, a.Dk, w, lane);
-  sv.init(vp, a.vn, a.Dv, w, lane);
-  sk.load(kbuf[0], 0, n, a.kn, w);
-  sv.load(vbuf[0], 0, n, a.vn, w);
+  sk.init(kp + part * BK * a.kn, a.kn, a.Dk, w, lane);
+  sv.init(vp + part * BK * a.vn, a.vn, a.Dv, w, lane);
+  sk.template load<G>(kbuf, part * BK, n, a.kn, w);
+  sv.template load<G>(vbuf, part * BK, n, a.vn, w);
   const int64_t row = q0 + 32 * w + n32;  // of the sequence
   const bool live = row < n;
   const bool flip = a.scale < 0.f;  // scores of -q and the scale's size
@@ -419,8 +445,8 @@ __global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
 
   const auto step = [&](int i, auto masked_of) __attribute__((always_inline)) {
     constexpr bool masked = decltype(masked_of)::value;
-    const char* kl = reinterpret_cast<const char*>(kbuf[i & 1]);
-    const char* vl = reinterpret_cast<const char*>(vbuf[i & 1]);
+    const char* kl = reinterpret_cast<const char*>(kbuf + (G == 1 ? i & 1 : i / G & 1) * kKeys);
+    const char* vl = reinterpret_cast<const char*>(vbuf + (G == 1 ? i & 1 : i / G & 1) * kValues);
     const int seen = masked ? (int)(row - (int64_t)i * BK) : 0;  // the last key of the step that the row sees
     f32x16 S[2];
 #pragma unroll
@@ -502,12 +528,13 @@ __global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
       }
     }
   };
-  for (int i = 0; i < steps; ++i) {
+  for (int it = 0; it * G < steps; ++it) {
+    const int i = it * G + part;
     lds_copies_done();  // this wavefront's rows of the step are in LDS
     __syncthreads();
-    if (i + 1 < steps) {
-      sk.load(kbuf[(i + 1) & 1], (int64_t)(i + 1) * BK, n, a.kn, w);
-      sv.load(vbuf[(i + 1) & 1], (int64_t)(i + 1) * BK, n, a.vn, w);
+    if (i + G < steps) {
+      sk.template load<G>(kbuf + ((it + 1) & 1) * kKeys, (int64_t)(i + G) * BK, n, a.kn, w);
+      sv.template load<G>(vbuf + ((it + 1) & 1) * kValues, (int64_t)(i + G) * BK, n, a.vn, w);
     }
     if (i >= mine) continue;  // every key is behind this wavefront's rows
     if ((int64_t)(i + 1) * BK <= q0 + 32 * w)
@@ -517,6 +544,34 @@ __global__ __launch_bounds__(kThreads, 2) void forward16(Args a) {
   }
   settle(O);
   l += __shfl_xor(l, 32);
+  if (G > 1) {
+    // The other part's sums, through LDS, to the larger maximum of the two.
+    f32x4* sums = reinterpret_cast<f32x4*>(lds) + w * (4 * VT * 64);
+    float2* ends = reinterpret_cast<float2*>(reinterpret_cast<f32x4*>(lds) + kWaves * 4 * VT * 64) + w * 64;
+    __syncthreads();  // what lds held is read
+    if (part == 1) {
+#pragma unroll
+      for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          sums[(vt * 4 + r) * 64 + lane] = f32x4{O[vt][4 * r], O[vt][4 * r + 1], O[vt][4 * r + 2], O[vt][4 * r + 3]};
+      ends[lane] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const float2 y = ends[lane];
+    const float top = fmaxf(m, y.x), base = top == -INFINITY ? 0.f : top;
+    const float f0 = exp2_fast(m - base), f1 = exp2_fast(y.x - base);
+    l = l * f0 + y.y * f1;
+#pragma unroll
+    for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 x = sums[(vt * 4 + r) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[vt][4 * r + i] = O[vt][4 * r + i] * f0 + x[i] * f1;
+      }
+  }
   if (!live) return;
   T* p = (T*)a.o + at.rows.batch * a.ob + h * a.oh + (at.rows.first + row) * a.on;
   const float il = 1.f / l;
@@ -587,7 +642,10 @@ extern "C" int kattn_fwd(const kattn_problem* p, void* o, const int64_t* o_strid
     const auto with = [&](auto ks, auto vt) {
       constexpr int KS = decltype(ks)::value, VT = decltype(vt)::value;
       if constexpr (sizeof(T) == 2)
-        forward16<T, KS, VT><<<dim3((unsigned)(a.tiles * a.H)), kThreads, 0, s>>>(a);
+        if (a.tiles * a.H <= 512)
+          forward16<T, KS, VT, 2><<<dim3((unsigned)(a.tiles * a.H)), kThreads * 2, 0, s>>>(a);
+        else
+          forward16<T, KS, VT, 1><<<dim3((unsigned)(a.tiles * a.H)), kThreads, 0, s>>>(a);
       else
         forward<T, KS, VT><<<dim3((unsigned)a.tiles, a.H), kThreads, 0, s>>>(a);
     };
