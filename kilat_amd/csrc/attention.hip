@@ -345,6 +345,13 @@ struct Stage {
   }
 };
 
+// The larger of x in this lane and in the one 32 from it.
+__device__ __forceinline__ float max_of_halves(float x) {
+  const unsigned y = __float_as_uint(x);
+  const auto z = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
+}
+
 // The halves of a word that are infinite or NaN, as masks of 16 bits.
 template <typename T>
 __device__ __forceinline__ unsigned not_finite(unsigned x) {
@@ -352,22 +359,24 @@ __device__ __forceinline__ unsigned not_finite(unsigned x) {
   return (((x & 0x7fff7fffu) + top) >> 15 & 0x00010001u) * 0xffffu;
 }
 
-// The tile that the `order`-th workgroup of a head takes in a packed batch of up to 64 sequences: the longest
-// sequence's first, each sequence's last tile first, so that what is left at the end is
-// short.  (-1: there are no more.)  A lane has a sequence.
-__device__ __forceinline__ int64_t longest_first(const Args& a, int64_t order, int lane) {
+// What the `order`-th workgroup of a head takes in a packed batch of up to 64 sequences: the longest
+// sequence's tiles first, each sequence's last tile first, so that what is left at the end
+// is short.  A lane has a sequence.
+__device__ __forceinline__ TileOf longest_first(const Args& a, int64_t order, int lane) {
   const Rows rows = lane < a.sequences ? rows_of(a.cu, lane, a.N) : Rows{0, 0, 0};
-  const int tiles = (int)((rows.n + BQ - 1) / BQ);
-  int before = 0;  // tiles of longer sequences
+  const int tiles = (int)((rows.n + BQ - 1) / BQ);  // (fewer than 2^31)
+  int before = 0;                                   // tiles of longer sequences
   for (int s = 0; s < (int)a.sequences; ++s) {
     const int other = __builtin_amdgcn_readlane(tiles, s);
     before += other > tiles || (other == tiles && s < lane) ? other : 0;
   }
   const unsigned long long found = __ballot(order >= before && order < before + tiles);
-  if (!found) return -1;
-  const int64_t tile = rows.first / BQ + lane + (before + tiles - 1 - order);
-  const int at = __ffsll(found) - 1;
-  return __builtin_amdgcn_readlane((int)tile, at);  // (tiles are fewer than 2^31)
+  const int s = found ? __ffsll(found) - 1 : 0;
+  const auto of = [&](int64_t x) {
+    return (int64_t)(((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), s) << 32) |
+                     (unsigned)__builtin_amdgcn_readlane((int)x, s));
+  };
+  return TileOf{s, found ? of(before + tiles - 1 - order) : 0, Rows{of(rows.first), found ? of(rows.n) : 0, 0}};
 }
 
 template <typename T, int KS, int VT, int G>
@@ -393,11 +402,7 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
   const int part = G == 1 ? 0 : wave_index() / kWaves, w = wave_index() % kWaves;  // steps part, part + G, ...; rows 32w..
   T *kbuf = lds + part * 2 * (kKeys + kValues), *vbuf = kbuf + 2 * kKeys;
   zero_outside<BQ>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, tid, kThreads * G);
-  if (a.cu && a.sequences <= 64) {
-    tile = longest_first(a, order, lane);
-    if (tile < 0) return;
-  }
-  const TileOf at = tile_of<BQ>(a.cu, a.sequences, tile, a.N);
+  const TileOf at = a.cu && a.sequences <= 64 ? longest_first(a, order, lane) : tile_of<BQ>(a.cu, a.sequences, tile, a.N);
   const int64_t q0 = at.index * BQ, n = at.rows.n;
   if (n <= q0) return;
   const T* kp = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + at.rows.first * a.kn;
@@ -467,7 +472,7 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
         if (masked) S[t][r] = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) <= seen ? S[t][r] : -INFINITY;
         top = fmaxf(top, S[t][r]);
       }
-    top = fmaxf(top, __shfl_xor(top, 32)) * to2;
+    top = max_of_halves(top) * to2;
     if (masked) top = seen < 0 ? -INFINITY : top;  // (to2 may be 0)
     // The maximum that is subtracted may be up to 8 (in powers of 2) below the true one: sums stay
     // far from 32 bits' end, and the rescaling of earlier sums is rare.

@@ -222,25 +222,29 @@ __device__ __forceinline__ int64_t first_tile(const int32_t* cu, int64_t s, cons
   return cu ? r.first / C + s : s * ((N + C - 1) / C);
 }
 
-// Tile `tile`, by bisection; rows.n <= index * C where it is none.
+// Tile `tile`; rows.n <= index * C where it is none.  A wavefront probes 64 sequences at a time: one round of
+// loads for up to 64 of them, two for up to 4096 (bisection takes six and twelve, one behind the
+// other, of a microsecond or so each where the offsets are not in the L2).
 template <int C>
 __device__ __forceinline__ TileOf tile_of(const int32_t* cu, int64_t sequences, int64_t tile, int64_t N) {
   int64_t s;
   if (!cu) {
     s = (unsigned)tile / (unsigned)((N + C - 1) / C);  // (tiles are fewer than 2^31)
   } else {
-    int64_t lo = 0, hi = sequences;  // the last s whose first tile is not behind `tile`
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if (clamp_row(cu[mid], N) / C + mid <= tile)
-        lo = mid;
-      else
-        hi = mid;
+    int64_t lo = 0, count = sequences;  // the last s whose first tile is not behind `tile` is one of these
+    const int lane = threadIdx.x & 63;
+    while (count > 1) {
+      const int64_t step = (count + 63) / 64, at = lane * step;
+      const bool ahead = at < count && clamp_row(cu[lo + (at < count ? at : 0)], N) / C + lo + at <= tile;
+      const int last = 63 - __clzll(__ballot(lane == 0 || ahead));
+      lo += last * step;
+      count = count - last * step < step ? count - last * step : step;
     }
     s = lo;
   }
   const Rows r = rows_of(cu, s, N);
-  return TileOf{s, tile - first_tile<C>(cu, s, r, N), r};
+  const int64_t index = tile - first_tile<C>(cu, s, r, N);
+  return index < 0 ? TileOf{s, 0, Rows{r.first, 0, r.batch}} : TileOf{s, index, r};  // (before the first sequence)
 }
 
 template <int C>
