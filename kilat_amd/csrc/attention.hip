@@ -302,13 +302,21 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
 // 16-byte chunks; a row's chunks are permuted by an exclusive or with its number, so
 // that neither the 32 rows that a key operand reads nor the eight that a value
 // operand reads lie in the same banks.  Values are transposed by the LDS read.
-template <int CPR>
+template <int CPR, bool VALUES>
 __device__ __forceinline__ int swizzle(int row) {
-  return CPR == 16 ? row & 15 : (row >> 1) & 7;
+  if (VALUES) return CPR == 16 ? (row & 3) << 2 : (row & 2) << 1;  // four rows by four adjacent chunks
+  return CPR == 16 ? row & 15 : (row >> 1) & 7;                    // 16 rows by one chunk
+}
+
+// The halves of a word that are infinite or NaN, as masks of 16 bits.
+template <typename T>
+__device__ __forceinline__ unsigned not_finite(unsigned x) {
+  constexpr unsigned top = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
+  return (((x & 0x7fff7fffu) + top) >> 15 & 0x00010001u) * 0xffffu;
 }
 
 // One wavefront's share of a tile of 64 rows of CPR chunks: NL instructions of 64 chunks.
-template <typename T, int CPR>
+template <typename T, int CPR, bool VALUES>
 struct Stage {
   static constexpr int NL = CPR / kWaves;
   const T* p[NL];
@@ -319,7 +327,7 @@ struct Stage {
     for (int i = 0; i < NL; ++i) {
       const int c = (w * NL + i) * 64 + lane, chunk = c % CPR;
       row[i] = c / CPR;
-      const int d = (chunk ^ swizzle<CPR>(row[i])) * 8;
+      const int d = (chunk ^ swizzle<CPR, VALUES>(row[i])) * 8;
       on[i] = d < width;
       p[i] = base + row[i] * stride + d;
     }
@@ -343,6 +351,19 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < NL; ++i) p[i] += G * BK * stride;
   }
+  // Zeroes what is not finite in this wavefront's share; whether there was any.
+  __device__ __forceinline__ bool clean(T* at, int w, int lane) {
+    unsigned bad = 0;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      uint4* x = reinterpret_cast<uint4*>(at + (w * NL + i) * 512 + lane * 8);
+      const uint4 y = *x;
+      const unsigned a = not_finite<T>(y.x), b = not_finite<T>(y.y), c = not_finite<T>(y.z), d = not_finite<T>(y.w);
+      if (a | b | c | d) *x = make_uint4(y.x & ~a, y.y & ~b, y.z & ~c, y.w & ~d);
+      bad |= a | b | c | d;
+    }
+    return __any(bad);
+  }
 };
 
 // The larger of x in this lane and in the one 32 from it.
@@ -350,13 +371,6 @@ __device__ __forceinline__ float max_of_halves(float x) {
   const unsigned y = __float_as_uint(x);
   const auto z = __builtin_amdgcn_permlane32_swap(y, y, false, false);
   return fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
-}
-
-// The halves of a word that are infinite or NaN, as masks of 16 bits.
-template <typename T>
-__device__ __forceinline__ unsigned not_finite(unsigned x) {
-  constexpr unsigned top = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
-  return (((x & 0x7fff7fffu) + top) >> 15 & 0x00010001u) * 0xffffu;
 }
 
 // What the `order`-th workgroup of a head takes in a packed batch of up to 64 sequences: the longest
@@ -385,6 +399,7 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
   constexpr int KC = 2 * KS, VC = 4 * VT;  // chunks of a row
   constexpr int kKeys = BK * KC * 8, kValues = BK * VC * 8;
   __shared__ __align__(16) T lds[G * 2 * (kKeys + kValues)];
+  __shared__ int odd[G][2];  // the last step with a masked key in the buffer and a value that is not finite
   // Workgroups go to the eight XCDs in turn.  With a multiple of eight heads each XCD has heads of
   // its own, so the keys that its workgroups read at the same time are the same; the tiles
   // with the most keys go first.
@@ -411,8 +426,8 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
     for (int i = tid; i < G * 2 * BK * (KC + VC); i += kThreads * G) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
-  Stage<T, KC> sk;
-  Stage<T, VC> sv;
+  Stage<T, KC, false> sk;
+  Stage<T, VC, true> sv;
   sk.init(kp + part * BK * a.kn, a.kn, a.Dk, w, lane);
   sv.init(vp + part * BK * a.vn, a.vn, a.Dv, w, lane);
   sk.template load<G>(kbuf, part * BK, n, a.kn, w);
@@ -431,20 +446,23 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
       const unsigned sign = flip ? 0x80008000u : 0u;
       y = left > 0 ? make_uint4(y.x ^ sign, y.y ^ sign, y.z ^ sign, y.w ^ sign) : make_uint4(0, 0, 0, 0);
       q[s] = __builtin_bit_cast(V8, y);
+      if (a.scale == 0.f) q[s] *= (T)0.f;  // (scores of 0, or NaN: `to2` is 1 then)
     }
   }
   // Where this lane reads: key operands, row n32 of a tile of 32, chunk 2s + half; value operands, by
   // 16 lanes, four keys (of half's four) of 16 channels.
-  const int kat = n32 * KC * 16, kx = half ^ swizzle<KC>(n32);
+  const int kat = n32 * KC * 16, kx = half ^ swizzle<KC, false>(n32);
   const int j = lane & 15, vrow = 4 * half + (j >> 2);
-  const int vat = vrow * VC * 16 + (j & 1) * 8, vx = (2 * ((lane >> 4) & 1) + ((j >> 1) & 1)) ^ swizzle<VC>(vrow);
+  const int vat = vrow * VC * 16 + (j & 1) * 8, vx = (2 * ((lane >> 4) & 1) + ((j >> 1) & 1)) ^ swizzle<VC, true>(vrow);
   f32x16 O[VT];
 #pragma unroll
   for (int t = 0; t < VT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) O[t][r] = 0.f;
   float m = -INFINITY, l = 0.f;
-  const float to2 = fabsf(a.scale) * 1.44269504088896340736f;  // scores in powers of 2
+  if (tid < 2 * G) odd[tid / 2][tid % 2] = -1;
+  __syncthreads();
+  const float to2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896340736f;  // scores in powers of 2
   const int64_t last = q0 + BQ < n ? q0 + BQ : n;
   const int steps = (int)((last + BK - 1) / BK), mine = (int)((q0 + 32 * w + 32 + BK - 1) / BK);  // of this wavefront's rows
 
@@ -452,7 +470,7 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
     constexpr bool masked = decltype(masked_of)::value;
     const char* kl = reinterpret_cast<const char*>(kbuf + (G == 1 ? i & 1 : i / G & 1) * kKeys);
     const char* vl = reinterpret_cast<const char*>(vbuf + (G == 1 ? i & 1 : i / G & 1) * kValues);
-    const int seen = masked ? (int)(row - (int64_t)i * BK) : 0;  // the last key of the step that the row sees
+    const int seen = masked ? (int)(row - (int64_t)i * BK) : 0, upto = seen - 4 * half;  // the last key that the row sees
     f32x16 S[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -469,11 +487,10 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        if (masked) S[t][r] = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3) <= seen ? S[t][r] : -INFINITY;
+        if (masked) S[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) <= upto ? S[t][r] : -INFINITY;
         top = fmaxf(top, S[t][r]);
       }
     top = max_of_halves(top) * to2;
-    if (masked) top = seen < 0 ? -INFINITY : top;  // (to2 may be 0)
     // The maximum that is subtracted may be up to 8 (in powers of 2) below the true one: sums stay
     // far from 32 bits' end, and the rescaling of earlier sums is rare.
     // (Row by row: what one row's scores are changes no digit of another's result.)
@@ -486,7 +503,6 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
       m = m1;
     }
     const float base = m == -INFINITY ? 0.f : m;
-    unsigned bad = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -494,8 +510,7 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
         V8 p;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          float x = exp2_fast(fmaf(S[t][8 * s + r], to2, -base));
-          if (masked) x = 32 * t + 16 * s + 8 * (r >> 2) + 4 * half + (r & 3) <= seen ? x : 0.f;
+          const float x = exp2_fast(fmaf(S[t][8 * s + r], to2, -base));
           l += x;
           p[r] = (T)x;
         }
@@ -504,20 +519,15 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
           u32x2 y[2];
 #pragma unroll
           for (int b = 0; b < 2; ++b)
-            y[b] = read_transposed(vl + (32 * t + 16 * s + 8 * b) * VC * 16 + vat + ((vx ^ (4 * vt) ^ swizzle<VC>(8 * b)) << 4));
-          uint4 z = make_uint4(y[0].x, y[0].y, y[1].x, y[1].y);
-          if (masked) {
-            const unsigned bx = not_finite<T>(z.x), by = not_finite<T>(z.y), bz = not_finite<T>(z.z), bw = not_finite<T>(z.w);
-            bad |= bx | by | bz | bw;
-            z = make_uint4(z.x & ~bx, z.y & ~by, z.z & ~bz, z.w & ~bw);
-          }
+            y[b] = read_transposed(vl + (32 * t + 16 * s + 8 * b) * VC * 16 + vat + ((vx ^ (4 * vt)) << 4));
+          const uint4 z = make_uint4(y[0].x, y[0].y, y[1].x, y[1].y);
           O[vt] = mfma32(__builtin_bit_cast(V8, z), p, O[vt]);
         }
       }
     }
+    settle(O);
     if (masked) {
-      settle(O);
-      if (__any(bad)) {
+      if (__builtin_amdgcn_readfirstlane(odd[part][i / G & 1]) == i) {
         // Values that are not finite were taken as 0: they count for the rows from their own on only.
         const int64_t k0 = (int64_t)i * BK;
         for (int key = 0; key < BK; ++key)
@@ -536,13 +546,18 @@ __global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void 
   for (int it = 0; it * G < steps; ++it) {
     const int i = it * G + part;
     lds_copies_done();  // this wavefront's rows of the step are in LDS
+    // Where some row does not see some key, values that are not finite become 0 (0 times one is none
+    // either); each wavefront looks at the rows that it has copied.
+    if ((int64_t)(i + 1) * BK > q0 && sv.clean(vbuf + (G == 1 ? i & 1 : i / G & 1) * kValues, w, lane) && lane == 0)
+      odd[part][i / G & 1] = i;
     __syncthreads();
     if (i + G < steps) {
       sk.template load<G>(kbuf + ((it + 1) & 1) * kKeys, (int64_t)(i + G) * BK, n, a.kn, w);
       sv.template load<G>(vbuf + ((it + 1) & 1) * kValues, (int64_t)(i + G) * BK, n, a.vn, w);
     }
     if (i >= mine) continue;  // every key is behind this wavefront's rows
-    if ((int64_t)(i + 1) * BK <= q0 + 32 * w)
+    const int64_t end = (int64_t)(i + 1) * BK;
+    if (end <= q0 || (end <= q0 + 32 * w && __builtin_amdgcn_readfirstlane(odd[part][i / G & 1]) != i))
       step(i, Bool<false>());
     else
       step(i, Bool<true>());
