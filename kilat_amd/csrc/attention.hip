@@ -232,8 +232,8 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int64_t key = k0 + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (masked && key > row) S[t][r] = -INFINITY;
         S[t][r] *= to2;
+        if (masked && key > row) S[t][r] = -INFINITY;
         top = fmaxf(top, S[t][r]);
       }
     top = fmaxf(top, __shfl_xor(top, 32));
@@ -662,6 +662,9 @@ extern "C" int kattn_fwd(const kattn_problem* p, void* o, const int64_t* o_strid
     const auto with = [&](auto ks, auto vt) {
       constexpr int KS = decltype(ks)::value, VT = decltype(vt)::value;
       if constexpr (sizeof(T) == 2)
+        // Keys in two parts where no compute unit has more than two workgroups: 16 heads of 4096 rows (512
+        // workgroups), Dk = Dv = 64: 66 us, else 92; 128: 112 and 148.  With more, the units are full, and
+        // the joining counts: 12 heads of eight sequences of 1024 rows (768), 64: 40 us, else 32.
         if (a.tiles * a.H <= 512)
           forward16<T, KS, VT, 2><<<dim3((unsigned)(a.tiles * a.H)), kThreads * 2, 0, s>>>(a);
         else

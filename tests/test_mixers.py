@@ -186,6 +186,20 @@ def test_abi_rejects_bad_buffers(kdecay_lib):
         assert step(**kw) == code, kw
 
 
+def test_abi_takes_rows_of_whole_vectors_only(kdecay_lib):
+    """Head dims that are no multiples of 8, rows and bases off 16 bytes: refused by both headers' functions."""
+    st, fake, big = (ctypes.c_int64 * 4)(12800, 6400, 64, 1), ctypes.c_void_p(FAKE), ctypes.c_size_t(1 << 40)
+    off = (ctypes.c_int64 * 4)(12800, 6400, 68, 1)
+    for kw, code in ((dict(Dk=20), _lib.KDECAY_ESHAPE), (dict(Dv=12), _lib.KDECAY_ESHAPE), (dict(q=FAKE + 2), _lib.KDECAY_ELAYOUT),
+                     (dict(k=FAKE + 8), _lib.KDECAY_ELAYOUT), (dict(vs=off), _lib.KDECAY_ELAYOUT),
+                     (dict(qs=off), _lib.KDECAY_ELAYOUT)):
+        assert kdecay_lib.kdelta_scan_fwd(ctypes.byref(problem(**kw)), fake, st, None, None, fake, big, None) == code, kw
+        assert kdecay_lib.kattn_fwd(ctypes.byref(problem(Attention, **kw)), fake, st, None) == code, kw
+    assert kdecay_lib.kdelta_scan_fwd(ctypes.byref(problem()), fake, off, None, None, fake, big, None) == _lib.KDECAY_ELAYOUT
+    assert kdecay_lib.kattn_fwd(ctypes.byref(problem(Attention)), fake, off, None) == _lib.KDECAY_ELAYOUT
+    assert kdecay_lib.kattn_fwd(ctypes.byref(problem(Attention)), ctypes.c_void_p(FAKE + 4), st, None) == _lib.KDECAY_ELAYOUT
+
+
 # ---------------------------------------------------------------------------
 # The oracles
 # ---------------------------------------------------------------------------
