@@ -914,39 +914,60 @@ __global__ __launch_bounds__(256) void join(Args a) {
 //            e^{G_64} <S, dS> + sum_j e^{G_64-G_j} k_j.(dS u_j)
 //     dg_i = sum of dG_i.. to the chunk's end
 // --------------------------------------------------------------------------
-template <typename T, int KB>
+// Few streams are cut into pieces as chain()'s are: numbered from the sequence's end, each first with nothing
+// behind it and with the identity's columns (MODE TRANS: N and M of dS <- M dS + N), join()ed.
+template <typename T, int KB, int MODE>
 __global__ __launch_bounds__(512) void chain_back(Args a) {
   constexpr int NI = kInputTerms<T>, NW = 4;
   __shared__ __bf16 Kf[4 * KB * NI * kFrag], Kt[4 * KB * NI * kFrag], Tf[kTri * NX * kFrag];
   __shared__ float vecs[2][V_CHAIN * C];
-  const int64_t seq = blockIdx.x;
+  const int pieces = MODE == TRANS ? a.segs - 1 : a.segs;
+  const int64_t seq = blockIdx.x / pieces;
+  const int seg = blockIdx.x % pieces;
   const int h = blockIdx.y, hk = h / a.group;
   const int wave = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const Rows rows = rows_of(a.cu, seq, a.N);
-  const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), nch = (rows.n + C - 1) / C;
+  const int64_t tile0 = first_tile<C>(a.cu, seq, rows, a.N), all = (rows.n + C - 1) / C;
+  const int64_t each = a.segs == 1 ? all : ((unsigned)all + a.segs - 1) / (unsigned)a.segs;  // chunks of a piece
+  const int64_t low = (a.segs - 1 - seg) * each, first = low < all ? low : all, nch = first + each < all ? first + each : all;
+  const int zv = (a.groups + NW - 1) / NW;
+  const bool unit = MODE == TRANS && (int)blockIdx.z >= zv;
+  if (unit && seg == 0) return;
+  const int64_t piece = (seq * a.H + h) * a.segs + seg;
   if (wave < NW) {
-    const int cg = blockIdx.z * NW + wave, col = 16 * cg + m;
-    const bool in = col < a.Dv, any = cg < a.groups;
+    const int cg = ((int)blockIdx.z - (unit ? zv : 0)) * NW + wave, col = 16 * cg + m;
+    const bool in = !unit && col < a.Dv, any = cg < (unit ? 2 * KB : a.groups);
     f32x4 S[2 * KB], Y[4], Z[2 * KB];
 #pragma unroll
-    for (int dt = 0; dt < 2 * KB; ++dt)
+    for (int dt = 0; dt < 2 * KB; ++dt) {
+      Z[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (MODE != TRANS && seg > 0) {
+        S[dt] = *reinterpret_cast<const f32x4*>(a.seg_s + ((piece * a.groups + (any ? cg : 0)) * 2 * KB + dt) * 256 + lane * 4);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = channel(dt, 4 * g + i);
-        S[dt][i] = a.d_final && in && d < a.Dk ? a.d_final[((seq * a.H + h) * a.Dk + d) * a.Dv + col] : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          const int d = channel(dt, 4 * g + i);
+          S[dt][i] = unit ? (d == col ? 1.f : 0.f)
+                     : a.d_final && seg == 0 && in && d < a.Dk ? a.d_final[((seq * a.H + h) * a.Dk + d) * a.Dv + col]
+                                                               : 0.f;
+        }
       }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) Y[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     const auto fetch = [&](int64_t c) __attribute__((always_inline)) {
+      if (unit) return;  // (dO is none of M's)
       const int64_t at = ((tile0 + c) * a.H + h) * a.groups + (any ? cg : 0);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) Y[mt] = *reinterpret_cast<const f32x4*>(a.ys + (at * 4 + mt) * 256 + lane * 4);
 #pragma unroll
       for (int dt = 0; dt < 2 * KB; ++dt) Z[dt] = *reinterpret_cast<const f32x4*>(a.zs + (at * 2 * KB + dt) * 256 + lane * 4);
     };
-    if (nch) {
+    if (first < nch) {
       fetch(nch - 1);
       lds_barrier();
     }
-    for (int64_t c = nch - 1; c >= 0; --c) {
+    for (int64_t c = nch - 1; c >= first; --c) {
       const int64_t tile = tile0 + c;
       const float* vec = vecs[c & 1];
       f32x4 X[4];
@@ -954,7 +975,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
         Terms<NX> s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
-        keep_state<KB>(a.dstates + planes_of<KB>(a, tile, h, cg >> 1), cg, m, g, s);
+        if (MODE != TRANS) keep_state<KB>(a.dstates + planes_of<KB>(a, tile, h, cg >> 1), cg, m, g, s);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) X[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -979,7 +1000,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
         for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(whole, S[dt][i], Z[dt][i]);
-        if (c) fetch(c - 1);
+        if (c > first) fetch(c - 1);
         const Terms<NX> u[2] = {split<NX>(X[0], X[1]), split<NX>(X[2], X[3])};
         f32x4 R[4];
         {
@@ -995,7 +1016,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
           products<2>(y, u[0], R);
         }
         settle(R);
-        {
+        if (MODE != TRANS) {
           const Terms<NX> r[2] = {split<NX>(R[0], R[1]), split<NX>(R[2], R[3])};
           keep_rows(a.drs + planes_of<2>(a, tile, h, cg >> 1), cg, m, g, r);
         }
@@ -1013,7 +1034,19 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
       }
       lds_barrier();
     }
-    if (a.d_init) {
+    if (MODE == TRANS) {
+      if (!any) return;
+      if (unit) {
+        Terms<NX> s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = split<NX>(S[2 * kb], S[2 * kb + 1]);
+        keep_state<KB>(a.seg_m + (piece * KB + (cg >> 1)) * (int64_t)(NX * 32 * 32 * KB), cg, m, g, s);
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < 2 * KB; ++dt)
+          *reinterpret_cast<f32x4*>(a.seg_n + ((piece * a.groups + cg) * 2 * KB + dt) * 256 + lane * 4) = S[dt];
+      }
+    } else if (a.d_init && seg + 1 == a.segs) {
 #pragma unroll
       for (int dt = 0; dt < 2 * KB; ++dt)
 #pragma unroll
@@ -1024,7 +1057,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
     }
     return;
   }
-  if (!nch) return;
+  if (first >= nch) return;
   // A feeder: tokens 16w + m of each chunk, as in chain().
   const int w = wave - NW, t = 16 * w + m, ft = threadIdx.x - 64 * NW;
   constexpr int TP = (kTri * NX + 3) / 4;
@@ -1057,7 +1090,7 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
   fetch(nch - 1);
   put_keys(nch - 1);
   lds_barrier();
-  for (int64_t c = nch - 1; c >= 0; --c) {
+  for (int64_t c = nch - 1; c >= first; --c) {
 #pragma unroll
     for (int x = 0; x < TP; ++x)
       if (4 * x + 4 <= kTri * NX || w + 4 * x < kTri * NX) *reinterpret_cast<bf16x8*>(Tf + (w + 4 * x) * kFrag + lane * 8) = tr[x];
@@ -1073,9 +1106,9 @@ __global__ __launch_bounds__(512) void chain_back(Args a) {
         *reinterpret_cast<u32x2*>(Kt + (((2 * kb + x / NI) * 2 + (w >> 1)) * NI + x % NI) * kFrag + lane * 8 + 4 * (w & 1)) = r;
       }
     }
-    if (c) fetch(c - 1);
+    if (c > first) fetch(c - 1);
     lds_barrier();
-    if (c) put_keys(c - 1);
+    if (c > first) put_keys(c - 1);
     lds_barrier();
   }
 }
@@ -1441,12 +1474,12 @@ constexpr int chain_waves(int element_size, int KB) { return element_size == 2 |
 // workgroups as a state has columns of its own), a join of 1 to 3 us per piece and two launches.
 // Measured (us, whole / pieces): B=1 H=16 N=65536 D=128 bf16 4212 / 1461 with 8, 1896 with 4, 1653 with 16;
 // B=8 H=6 N=1024 D=64 64 / 52 with 4, 69 with 6; B=4 H=16 N=2047 D=80 fp16 202 / 179
-// with 2, 221 with 4; B=2 H=6 N=1024 D=64 float32 (with the backward) 266 / 163 with 8.  (A packed batch: by the
-// mean length.)
-int pieces_of(const kdelta_problem* p) {
+// with 2, 221 with 4; B=2 H=6 N=1024 D=64 float32 (with the backward) 266 / 163 with 8.  The backward's chain, the same call:
+// 132 then 157; B=8 H=12 N=4096 D=64 bf16, 2 pieces: 1055 and 1084. (A packed batch: by the mean length.)
+int pieces_of(const kdelta_problem* p, bool backward) {
   constexpr double kCus = 256, kPass = 0.65, kFixed = 4;
   if (!p->sequences) return 1;
-  const int64_t KB = (p->Dk + 31) / 32, NW = chain_waves(p->dtype == KDECAY_F32 ? 4 : 2, (int)KB);
+  const int64_t KB = (p->Dk + 31) / 32, NW = backward ? 4 : chain_waves(p->dtype == KDECAY_F32 ? 4 : 2, (int)KB);
   const int64_t zv = (2 * ((p->Dv + 31) / 32) + NW - 1) / NW, zk = (2 * KB + NW - 1) / NW;
   const int64_t chunks = (p->N / (p->cu_seqlens ? p->sequences : 1) + C - 1) / C;
   const double streams = (double)p->sequences * p->H, join = 0.75 * KB;
@@ -1466,7 +1499,7 @@ struct Sizes {  // bytes
   size_t vecs, tris, back_tris, ys, zs, states, rows, seg_n, seg_m;
 };
 
-Sizes sizes_of(const kdelta_problem* p) {
+Sizes sizes_of(const kdelta_problem* p, bool backward) {
   const size_t heads = (size_t)tiles_of(p) * p->H, KB = (p->Dk + 31) / 32, blocks = blocks_of(p);
   Sizes s;
   s.vecs = up256(heads * V_COUNT * C * 4);
@@ -1476,7 +1509,7 @@ Sizes sizes_of(const kdelta_problem* p) {
   s.zs = up256(heads * 2 * blocks * 2 * KB * 256 * 4);
   s.states = up256(heads * blocks * NX * 32 * 32 * KB * 2);
   s.rows = up256(heads * blocks * NX * 32 * C * 2);
-  const size_t segs = pieces_of(p), pieces = segs > 1 ? (size_t)p->sequences * p->H * segs : 0;
+  const size_t segs = pieces_of(p, backward), pieces = segs > 1 ? (size_t)p->sequences * p->H * segs : 0;
   s.seg_n = up256(pieces * 2 * blocks * 2 * KB * 256 * 4);
   s.seg_m = up256(pieces * KB * NX * 32 * 32 * KB * 2);
   return s;
@@ -1519,24 +1552,23 @@ Args args_of(const kdelta_problem* p, void* workspace, const float* saved, bool 
   a.scale = p->scale;
   a.blocks = (int)blocks_of(p);
   a.groups = 2 * a.blocks;
-  const Sizes s = sizes_of(p);
+  const Sizes s = sizes_of(p, backward);
   char* w = (char*)workspace;
   a.vecs = (float*)w, w += s.vecs;
   a.tris = (__bf16*)w;
-  a.segs = 1;
+  a.segs = pieces_of(p, backward);
   if (!backward) {
     w += s.tris;
-    a.segs = pieces_of(p);
-    a.seg_n = (float*)w, w += s.seg_n;
-    a.seg_s = (float*)w, w += s.seg_n;
-    a.seg_m = (__bf16*)w;
   } else {
     w += s.back_tris;
     a.ys = (float*)w, w += s.ys;
     a.zs = (float*)w, w += s.zs;
     a.dstates = (__bf16*)w, w += s.states;
-    a.drs = (__bf16*)w;
+    a.drs = (__bf16*)w, w += s.rows;
   }
+  a.seg_n = (float*)w, w += s.seg_n;
+  a.seg_s = (float*)w, w += s.seg_n;
+  a.seg_m = (__bf16*)w;
   a.states = (__bf16*)saved;
   a.us = saved ? (__bf16*)((char*)saved + s.states) : nullptr;
   return a;
@@ -1573,19 +1605,19 @@ using namespace kd::delta;
 
 extern "C" size_t kdelta_scan_workspace_bytes(const kdelta_problem* p) {
   if (check(p)) return 0;
-  const Sizes s = sizes_of(p);
+  const Sizes s = sizes_of(p, false);
   return s.vecs + s.tris + 2 * s.seg_n + s.seg_m;
 }
 
 extern "C" size_t kdelta_scan_bwd_workspace_bytes(const kdelta_problem* p) {
   if (check(p)) return 0;
-  const Sizes s = sizes_of(p);
-  return s.vecs + s.back_tris + s.ys + s.zs + s.states + s.rows;
+  const Sizes s = sizes_of(p, true);
+  return s.vecs + s.back_tris + s.ys + s.zs + s.states + s.rows + 2 * s.seg_n + s.seg_m;
 }
 
 extern "C" size_t kdelta_scan_saved_floats(const kdelta_problem* p) {
   if (check(p)) return 0;
-  const Sizes s = sizes_of(p);
+  const Sizes s = sizes_of(p, false);
   return (s.states + s.rows) / 4;
 }
 
@@ -1670,7 +1702,15 @@ extern "C" int kdelta_scan_bwd(const kdelta_problem* p, const void* d_o, const i
         prep<T, KB, true><<<dim3((unsigned)a.tiles, a.H), 256, 0, s>>>(a);
         if (const int rc = hip_check("kdelta prep launch")) return rc;
       }
-      chain_back<T, KB><<<chain_grid(a, 4), 512, 0, s>>>(a);
+      const dim3 grid = chain_grid(a, 4);
+      if (a.segs > 1) {
+        const dim3 pieces((unsigned)(a.sequences * (a.segs - 1)), a.H, grid.z + (2 * KB + 3) / 4);
+        chain_back<T, KB, TRANS><<<pieces, 512, 0, s>>>(a);
+        if (const int rc = hip_check("kdelta chain_back launch")) return rc;
+        join<KB><<<dim3((unsigned)a.sequences, a.H, (a.groups + 3) / 4), 256, 0, s>>>(a);
+        if (const int rc = hip_check("kdelta join launch")) return rc;
+      }
+      chain_back<T, KB, PLAIN><<<grid, 512, 0, s>>>(a);
       if (const int rc = hip_check("kdelta chain_back launch")) return rc;
       if (!rows) return 0;
       if (a.group > 1)
