@@ -56,11 +56,13 @@ def gated_delta_scan(
     cu_seqlens: int32/int64 [S+1] on the device, non-decreasing, for a packed
     batch (B=1): sequence s is the rows cu_seqlens[s]..cu_seqlens[s+1], and the
     states are [S,H,Dk,Dv].  Its values are never read on the host.  Rows of no
-    sequence give zeros, in o and in the gradients.
+    sequence give zeros, in o and in the gradients.  (Its mean length decides into how
+    many pieces the sequences are cut.)
 
     Returns o ([B,H,N,Dv], v's dtype, laid out like v), and with
     return_final_state also the final states (float32).  Arithmetic is float32
-    whatever the dtype: o is rounded once.  A value that is not finite reaches
+    whatever the dtype (what reaches only a 16-bit o: to 2^-16), and o is rounded
+    once.  A value that is not finite reaches
     the tokens from its own on, in the columns and heads it reaches by the formula.
 
     With requires_grad on any input the result carries a backward (gradients of q,
@@ -113,7 +115,8 @@ def causal_attention(
     rows of no sequence give zeros.
 
     Returns o [B,H,N,Dv] of q's dtype, laid out like q.  Softmax statistics and
-    sums are float32.  A prefill's forward: inputs that require grad are refused.
+    sums are float32; of 16-bit inputs the probabilities are rounded to the type, as the
+    second product's operands.  No row sees a later one's values, finite or not.  A prefill's forward: inputs that require grad are refused.
     """
     _tensors(q=q, k=k, v=v)
     return _native().causal_attention(q, k, v, scale, cu_seqlens)
