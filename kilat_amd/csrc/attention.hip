@@ -117,17 +117,20 @@ struct Bool {
   static constexpr bool value = B;
 };
 
-// float32: rows pass registers, where they are split into terms.
+// float32: rows pass registers, where they are split into terms.  Six matrix instructions for one, and as many
+// vector instructions for the splits: 16 heads of 4096 rows, Dk = Dv = 64: 401 us, 86 TFLOP/s of
+// float32; 128: 912 us, 75 (a large product of torch's in float32 reaches 154).  Two workgroups per CU
+// where registers allow (Dv <= 64): 546 us with one.
 // KS: steps of 16 channels of q and k; VT: tiles of 32 channels of v.
 template <typename T, int KS, int VT>
-__global__ __launch_bounds__(kThreads) void forward(Args a) {
+__global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
   typedef typename Op<T>::E E;
   typedef typename Vec8<E>::half E4;
   constexpr int N = Op<T>::N;
   __shared__ E ks[N][2 * KS * kTile];  // keys: two tiles of 32 keys, KS steps
   __shared__ E vs[N][4 * VT * kTile];  // values, transposed: VT tiles of 32 channels, four steps of 16 keys
   __shared__ int odd;                  // a value of a step that masks keys is not finite
-  const int64_t tile = blockIdx.x;
+  const int64_t tile = a.tiles - 1 - blockIdx.x;  // a sequence's last rows, which have the most keys, first
   const int h = blockIdx.y, hk = h / a.group;
   const int tid = threadIdx.x, w = tid / 64, lane = tid & 63, n32 = lane & 31, half = lane >> 5;
   zero_outside<BQ>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, tid, kThreads);
@@ -158,13 +161,34 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
   const int64_t last = q0 + BQ < at.rows.n ? q0 + BQ : at.rows.n;
   for (int64_t k0 = 0; k0 < last; k0 += BK) {
     const bool masked = k0 + BK > q0;  // keys behind some row, or behind the sequence
+    // All of the step's loads first: one wait for memory.
+    constexpr int KI = BK * 2 * KS / kThreads, VI = BK / 4 * 8 * VT / kThreads;
+    Raw8<T> kr[KI];
+    Raw4<T> vr[VI][4];
+#pragma unroll
+    for (int x = 0; x < KI; ++x) {
+      const int i = tid + x * kThreads, key = i / (2 * KS), c = i % (2 * KS);
+      kr[x] = fetch8(kp, (k0 + key) * a.kn + 8 * c, k0 + key < at.rows.n ? a.Dk - 8 * c : 0);
+    }
+#pragma unroll
+    for (int x = 0; x < VI; ++x) {
+      const int i = tid + x * kThreads, kg = i / (8 * VT), c = (i % (8 * VT)) * 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t key = k0 + 4 * kg + j;
+        vr[x][j] = fetch4(vp, key * a.vn + c, key < at.rows.n ? a.Dv - c : 0);
+      }
+    }
     __syncthreads();
     if (tid == 0) odd = 0;
     // keys
-    for (int i = tid; i < BK * 2 * KS; i += kThreads) {
-      const int key = i / (2 * KS), c = i % (2 * KS);
+#pragma unroll
+    for (int z = 0; z < KI; ++z) {
+      const int i = tid + z * kThreads, key = i / (2 * KS), c = i % (2 * KS);
+      const bool there = k0 + key < at.rows.n && a.Dk > 8 * c;
       float x[8];
-      load_row8(kp, (k0 + key) * a.kn + 8 * c, k0 + key < at.rows.n ? a.Dk - 8 * c : 0, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = there ? (float)kr[z][j] : 0.f;
       const Operand<T> y = to_operand<T>(x);
       const int slot = ((key & 31) + 32 * (c & 1)) ^ (c & 15);
 #pragma unroll
@@ -173,13 +197,14 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
     }
     __syncthreads();
     // values: four keys of four channels at a time, transposed
-    for (int i = tid; i < (BK / 4) * 8 * VT; i += kThreads) {
-      const int kg = i / (8 * VT), c = (i % (8 * VT)) * 4;
+#pragma unroll
+    for (int z = 0; z < VI; ++z) {
+      const int i = tid + z * kThreads, kg = i / (8 * VT), c = (i % (8 * VT)) * 4;
       f32x4 x[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t key = k0 + 4 * kg + j;
-        x[j] = load4(vp, key * a.vn + c, key < at.rows.n ? a.Dv - c : 0);
+        x[j] = fetched<T>(vr[z][j], key < at.rows.n ? a.Dv - c : 0);
         if (masked) {
 #pragma unroll
           for (int d = 0; d < 4; ++d)
@@ -227,13 +252,13 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
       }
     }
     float top = -INFINITY;
+    const int upto = (int)(row - k0) - 4 * half;  // the last key that the row sees
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int64_t key = k0 + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
         S[t][r] *= to2;
-        if (masked && key > row) S[t][r] = -INFINITY;
+        if (masked) S[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) <= upto ? S[t][r] : -INFINITY;
         top = fmaxf(top, S[t][r]);
       }
     top = fmaxf(top, __shfl_xor(top, 32));
@@ -307,8 +332,7 @@ __global__ __launch_bounds__(kThreads) void forward(Args a) {
 // instructions, 32 of them exponentials at a quarter of the rate, for 16 (Dk = Dv = 64) or 32 (128)
 // matrix instructions.  16384 rows, 16 heads (4 key heads), 128, bfloat16: 1342 us, 820 TFLOP/s (a large matrix
 // product of torch's reaches 1222); eight sequences of 1024 rows, 6 heads, 64: 23.8 us, of which the
-// longest rows' 8 rounds of twice 64 keys take 12 and the launch 6.  Three workgroups per CU for 64 (168 registers)
-// against two: 72 and 80 us for a packed batch of 16384 rows.
+// longest rows' 8 rounds of twice 64 keys take 12 and the launch 6.
 template <int CPR, bool VALUES>
 __device__ __forceinline__ int swizzle(int row) {
   if (VALUES) return CPR == 16 ? (row & 3) << 2 : (row & 2) << 1;  // four rows by four adjacent chunks
@@ -401,7 +425,7 @@ __device__ __forceinline__ TileOf longest_first(const Args& a, int64_t order, in
 }
 
 template <typename T, int KS, int VT, int G>
-__global__ __launch_bounds__(kThreads * G, G == 1 && KS * VT <= 8 ? 3 : 2) void forward16(Args a) {
+__global__ __launch_bounds__(kThreads * G, 2) void forward16(Args a) {
   typedef typename Vec8<T>::type V8;
   constexpr int KC = 2 * KS, VC = 4 * VT;  // chunks of a row
   constexpr int kKeys = BK * KC * 8, kValues = BK * VC * 8;
