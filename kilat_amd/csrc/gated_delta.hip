@@ -213,8 +213,8 @@ __device__ __forceinline__ float fade(double x) {
 // and no difference becomes inf - inf.
 //
 // Bound by the latency of one workgroup's own steps (loads, K K', the inverse by tiles, stores) and, on
-// full grids, by memory: B=8 H=12 N=4096 D=64 bfloat16, 6144 tiles, takes 97 us for 290 MB
-// (3.0 TB/s), BWD 168 us for 460 MB; 768 tiles (one round of workgroups) take 18 us.
+// full grids, by memory: B=8 H=12 N=4096 D=64 bfloat16, 6144 tiles, takes 72 us for 290 MB
+// (4.0 TB/s), BWD 140 us for 460 MB (3.3); 768 tiles (one round of workgroups) take 14 us.
 template <typename T, int KB, bool BWD>
 __global__ __launch_bounds__(256) void prep(Args a) {
   constexpr int NI = kInputTerms<T>;
@@ -222,9 +222,8 @@ __global__ __launch_bounds__(256) void prep(Args a) {
   constexpr int kKeys = 4 * KB * NI * kFrag, kQt = 4 * KB * NX * kFrag, kDo = 8 * NI * kFrag;
   // K (and Q); BWD: later Q transposed and 64 columns of dO transposed
   __shared__ __align__(16) __bf16 kq[!BWD ? kKeys : 2 * kKeys > kQt + kDo ? 2 * kKeys : kQt + kDo];
-  __shared__ float As[C * LD], Ts[C * LD];
-  __shared__ double Gs[C];
-  __shared__ float bs[C];
+  __shared__ __align__(16) float As[C * LD], Ts[C * LD];
+  __shared__ __align__(16) float Gh[C], Gl[C], bs[C], es[C];  // G log2(e) as the sum of two, b, e^G
   const int64_t tile = blockIdx.x;
   const int h = blockIdx.y, hk = h / a.group;
   const int w = wave_index(), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -262,8 +261,6 @@ __global__ __launch_bounds__(256) void prep(Args a) {
       const double y = __shfl_up(G, d);
       if (lane >= d) G += y;
     }
-    Gs[lane] = G;
-    bs[lane] = b;
     const double all = __shfl(G, 63);
     float* vec = vec_of(a, tile, h);
     const float since = fade(G);
@@ -272,8 +269,10 @@ __global__ __launch_bounds__(256) void prep(Args a) {
     vec[V_SINCE * C + lane] = since;
     vec[V_LEFT * C + lane] = fade(all - G);
     const double G2 = G * 1.4426950408889634074;
-    vec[V_G * C + lane] = (float)G2;
-    vec[V_GLOW * C + lane] = (float)(G2 - (double)(float)G2);
+    const float high = (float)G2, low = (float)(G2 - (double)high);
+    vec[V_G * C + lane] = high;
+    vec[V_GLOW * C + lane] = low;
+    Gh[lane] = high, Gl[lane] = low, bs[lane] = b, es[lane] = since;
   }
   Terms<NI> kt[KB];
 #pragma unroll
@@ -284,46 +283,46 @@ __global__ __launch_bounds__(256) void prep(Args a) {
     if constexpr (BWD) store_terms<NI>(kq + kKeys + (w * KB + kb) * NI * kFrag, lane, terms_of<T>(qr[kb], left));
   }
   __syncthreads();
-  // A for tokens i of this wavefront, lane m = column j (read by rows below).
-#pragma unroll
-  for (int jt = 0; jt < 4; ++jt) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (jt <= w) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) acc = product<2>(kt[kb], load_terms<NI>(kq + (jt * KB + kb) * NI * kFrag, lane), acc);
-      settle(acc);
-    }
-    const int j = 16 * jt + m;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int i = 16 * w + 4 * g + x;
-      As[i * LD + j] = j < i ? bs[i] * fade(Gs[i] - Gs[j]) * acc[x] : 0.f;
-    }
-  }
+  // A and P, with one e^{G_i - G_j} for both: lane m has this wavefront's token t as i and the rows of the
+  // result as j (BWD: t as j, rows as i).  Differences of the high parts are exact where they count, so an
+  // exponential is off by its own rounding (1 to 2 units of 2^-24) only.
   Terms<BWD ? NX : 1> pt[2] = {};  // BWD: P transposed
-  {  // P: rows i of this wavefront (BWD: transposed, rows j)
+  {
+    const float gh = Gh[t], gl = Gl[t], bt = bs[t];
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
       if (BWD ? kb2 < w / 2 : kb2 > w / 2) continue;
-      f32x4 p[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      f32x4 p[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, aa[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         Terms<NI> y[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) y[x] = load_terms<NI>(kq + (BWD ? kKeys : 0) + ((2 * kb2 + x) * KB + kb) * NI * kFrag, lane);
-        if constexpr (BWD)
-          products<2>(y, kt[kb], p);
-        else
-          products<2>(y, terms_of<T>(qr[kb], t < n ? a.Dk - 32 * kb - 8 * g : 0), p);
-      }
-      settle(p);
+        for (int x = 0; x < 2; ++x) y[x] = load_terms<NI>(kq + ((2 * kb2 + x) * KB + kb) * NI * kFrag, lane);
+        products<2>(y, kt[kb], aa);
+        if constexpr (BWD) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 2; ++x) y[x] = load_terms<NI>(kq + kKeys + ((2 * kb2 + x) * KB + kb) * NI * kFrag, lane);
+          products<2>(y, kt[kb], p);
+        } else {
+          products<2>(y, terms_of<T>(qr[kb], t < n ? a.Dk - 32 * kb - 8 * g : 0), p);
+        }
+      }
+      settle(p), settle(aa);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int o = 32 * kb2 + 16 * x + 4 * g;
+        const f32x4 oh = *reinterpret_cast<const f32x4*>(Gh + o), ol = *reinterpret_cast<const f32x4*>(Gl + o);
+        const f32x4 ob = *reinterpret_cast<const f32x4*>(bs + o);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int other = 32 * kb2 + 16 * x + 4 * g + r, i = BWD ? other : t, j = BWD ? t : other;
-          p[x][r] = j <= i ? a.scale * fade(Gs[i] - Gs[j]) * p[x][r] : 0.f;
+          const int i = BWD ? o + r : t, j = BWD ? t : o + r;
+          const float d = BWD ? (oh[r] - gh) + (ol[r] - gl) : (gh - oh[r]) + (gl - ol[r]), e = exp2_fast(d);
+          p[x][r] = j <= i ? a.scale * e * p[x][r] : 0.f;
+          aa[x][r] = j < i ? (BWD ? ob[r] : bt) * e * aa[x][r] : 0.f;
+          if (BWD) As[i * LD + j] = aa[x][r];
         }
+        if (!BWD) *reinterpret_cast<f32x4*>(As + t * LD + o) = aa[x];
+      }
       if constexpr (BWD) {
         pt[kb2] = split<NX>(p[0], p[1]);
       } else {
@@ -393,7 +392,7 @@ __global__ __launch_bounds__(256) void prep(Args a) {
   }
   if constexpr (BWD) {
     __bf16 *Qt = kq, *Do = kq + kQt;
-    const f32x4 since = a.scale * f32x4{fade(Gs[16 * w + 4 * g]), fade(Gs[16 * w + 4 * g + 1]), fade(Gs[16 * w + 4 * g + 2]), fade(Gs[16 * w + 4 * g + 3])};
+    const f32x4 since = a.scale * *reinterpret_cast<const f32x4*>(es + 16 * w + 4 * g);
     // Q transposed, rows in the order of a state's.
     const bf16x8 ksel[2] = {selector(channel(0, m), g), selector(channel(1, m), g)};
     const bf16x8 vsel[2] = {selector(m, g), selector(16 + m, g)};
