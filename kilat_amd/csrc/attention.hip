@@ -22,19 +22,6 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kTile = 512;  // values of one operand tile (64 lanes of 8)
 
-// What the matrix instructions take for inputs of type T: 16-bit types as they are,
-// float32 as three bfloat16 terms (matrix.h), products kept to 2^-24.
-template <typename T>
-struct Op {
-  typedef T E;
-  static constexpr int N = 1, ORDER = 0;
-};
-template <>
-struct Op<float> {
-  typedef __bf16 E;
-  static constexpr int N = 3, ORDER = 2;
-};
-
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -42,48 +29,23 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-template <typename E>
+template <typename T>
 struct Vec8;
 template <>
 struct Vec8<__bf16> {
   typedef bf16x8 type;
-  typedef bf16x4 half;
 };
 template <>
 struct Vec8<_Float16> {
   typedef f16x8 type;
-  typedef _Float16 half __attribute__((ext_vector_type(4)));
 };
 
-// Eight values of an operand, by terms.
-template <typename T>
-struct Operand {
-  typedef typename Vec8<typename Op<T>::E>::type V;
-  V t[Op<T>::N];
-};
-
-template <typename T>
-__device__ __forceinline__ Operand<T> to_operand(const float (&x)[8]) {
-  Operand<T> r;
-  if constexpr (Op<T>::N == 1) {
+// A product of float32 operands as three bfloat16 terms each (matrix.h), kept to 2^-24.
+__device__ __forceinline__ f32x16 product32(const Terms<3>& a, const Terms<3>& b, f32x16 acc) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.t[0][i] = (T)x[i];
-  } else {
-    const Terms<3> s = split<3>(x);
+  for (int s = 2; s >= 0; --s)
 #pragma unroll
-    for (int i = 0; i < 3; ++i) r.t[i] = s.t[i];
-  }
-  return r;
-}
-
-template <typename T>
-__device__ __forceinline__ f32x16 product32(const Operand<T>& a, const Operand<T>& b, f32x16 acc) {
-  constexpr int N = Op<T>::N;
-#pragma unroll
-  for (int s = Op<T>::ORDER; s >= 0; --s)
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (s - i >= 0 && s - i < N) acc = mfma32(a.t[i], b.t[s - i >= 0 && s - i < N ? s - i : 0], acc);
+    for (int i = 0; i <= s; ++i) acc = mfma32(a.t[i], b.t[s - i], acc);
   return acc;
 }
 
@@ -103,8 +65,7 @@ struct Args {
 };
 
 // Eight elements from base + at, n of them there.
-template <typename T>
-__device__ __forceinline__ void load_row8(const T* base, int64_t at, int n, float (&x)[8]) {
+__device__ __forceinline__ void load_row8(const float* base, int64_t at, int n, float (&x)[8]) {
   const f32x4 a = load4(base, at, n), b = load4(base, at + 4, n - 4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
@@ -122,33 +83,31 @@ struct Bool {
 // float32; 128: 912 us, 75 (a large product of torch's in float32 reaches 154).  Two workgroups per CU
 // where registers allow (Dv <= 64): 546 us with one.
 // KS: steps of 16 channels of q and k; VT: tiles of 32 channels of v.
-template <typename T, int KS, int VT>
+template <int KS, int VT>
 __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
-  typedef typename Op<T>::E E;
-  typedef typename Vec8<E>::half E4;
-  constexpr int N = Op<T>::N;
-  __shared__ E ks[N][2 * KS * kTile];  // keys: two tiles of 32 keys, KS steps
-  __shared__ E vs[N][4 * VT * kTile];  // values, transposed: VT tiles of 32 channels, four steps of 16 keys
+  constexpr int N = 3;  // terms
+  __shared__ __bf16 ks[N][2 * KS * kTile];  // keys: two tiles of 32 keys, KS steps
+  __shared__ __bf16 vs[N][4 * VT * kTile];  // values, transposed: VT tiles of 32 channels, four steps of 16 keys
   __shared__ int odd;                  // a value of a step that masks keys is not finite
   const int64_t tile = a.tiles - 1 - blockIdx.x;  // a sequence's last rows, which have the most keys, first
   const int h = blockIdx.y, hk = h / a.group;
   const int tid = threadIdx.x, w = tid / 64, lane = tid & 63, n32 = lane & 31, half = lane >> 5;
-  zero_outside<BQ>(a.cu, a.sequences, tile, a.N, (T*)a.o + h * a.oh, a.on, a.Dv, tid, kThreads);
+  zero_outside<BQ>(a.cu, a.sequences, tile, a.N, (float*)a.o + h * a.oh, a.on, a.Dv, tid, kThreads);
   const TileOf at = tile_of<BQ>(a.cu, a.sequences, tile, a.N);
   const int64_t q0 = at.index * BQ;
   if (at.rows.n <= q0) return;
-  const T* kp = (const T*)a.k + at.rows.batch * a.kb + hk * a.kh + at.rows.first * a.kn;
-  const T* vp = (const T*)a.v + at.rows.batch * a.vb + hk * a.vh + at.rows.first * a.vn;
+  const float* kp = (const float*)a.k + at.rows.batch * a.kb + hk * a.kh + at.rows.first * a.kn;
+  const float* vp = (const float*)a.v + at.rows.batch * a.vb + hk * a.vh + at.rows.first * a.vn;
   const int64_t row = q0 + 32 * w + n32;  // of the sequence
   const bool live = row < at.rows.n;
-  Operand<T> q[KS];
+  Terms<3> q[KS];
   {
-    const T* p = (const T*)a.q + at.rows.batch * a.qb + h * a.qh + at.rows.first * a.qn;
+    const float* p = (const float*)a.q + at.rows.batch * a.qb + h * a.qh + at.rows.first * a.qn;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       float x[8];
       load_row8(p, row * a.qn + 16 * s + 8 * half, live ? a.Dk - 16 * s - 8 * half : 0, x);
-      q[s] = to_operand<T>(x);
+      q[s] = split<3>(x);
     }
   }
   f32x16 O[VT];
@@ -163,8 +122,8 @@ __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
     const bool masked = k0 + BK > q0;  // keys behind some row, or behind the sequence
     // All of the step's loads first: one wait for memory.
     constexpr int KI = BK * 2 * KS / kThreads, VI = BK / 4 * 8 * VT / kThreads;
-    Raw8<T> kr[KI];
-    Raw4<T> vr[VI][4];
+    Raw8<float> kr[KI];
+    Raw4<float> vr[VI][4];
 #pragma unroll
     for (int x = 0; x < KI; ++x) {
       const int i = tid + x * kThreads, key = i / (2 * KS), c = i % (2 * KS);
@@ -189,11 +148,11 @@ __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = there ? (float)kr[z][j] : 0.f;
-      const Operand<T> y = to_operand<T>(x);
+      const Terms<3> y = split<3>(x);
       const int slot = ((key & 31) + 32 * (c & 1)) ^ (c & 15);
 #pragma unroll
       for (int t = 0; t < N; ++t)
-        *reinterpret_cast<typename Operand<T>::V*>(&ks[t][((key >> 5) * KS + (c >> 1)) * kTile + slot * 8]) = y.t[t];
+        *reinterpret_cast<bf16x8*>(&ks[t][((key >> 5) * KS + (c >> 1)) * kTile + slot * 8]) = y.t[t];
     }
     __syncthreads();
     // values: four keys of four channels at a time, transposed
@@ -204,7 +163,7 @@ __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t key = k0 + 4 * kg + j;
-        x[j] = fetched<T>(vr[z][j], key < at.rows.n ? a.Dv - c : 0);
+        x[j] = fetched<float>(vr[z][j], key < at.rows.n ? a.Dv - c : 0);
         if (masked) {
 #pragma unroll
           for (int d = 0; d < 4; ++d)
@@ -219,18 +178,18 @@ __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
         float y[4] = {x[0][d], x[1][d], x[2][d], x[3][d]};
 #pragma unroll
         for (int t = 0; t < N; ++t) {
-          E4 e;
+          bf16x4 e;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (t + 1 < N) {
               const float u = upper_half(y[j]);
-              e[j] = (E)u;
+              e[j] = (__bf16)u;
               y[j] -= u;
             } else {
-              e[j] = (E)y[j];
+              e[j] = (__bf16)y[j];
             }
           }
-          *reinterpret_cast<E4*>(&vs[t][at8]) = e;
+          *reinterpret_cast<bf16x4*>(&vs[t][at8]) = e;
         }
       }
     }
@@ -243,12 +202,12 @@ __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
       for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        Operand<T> x;
+        Terms<3> x;
 #pragma unroll
         for (int y = 0; y < N; ++y)
-          x.t[y] = *reinterpret_cast<const typename Operand<T>::V*>(
+          x.t[y] = *reinterpret_cast<const bf16x8*>(
               &ks[y][(t * KS + s) * kTile + (lane ^ ((2 * s + half) & 15)) * 8]);
-        S[t] = product32<T>(x, q[s], S[t]);
+        S[t] = product32(x, q[s], S[t]);
       }
     }
     float top = -INFINITY;
@@ -281,14 +240,14 @@ __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const float x[8] = {p[8 * s], p[8 * s + 1], p[8 * s + 2], p[8 * s + 3], p[8 * s + 4], p[8 * s + 5], p[8 * s + 6], p[8 * s + 7]};
-        const Operand<T> pt = to_operand<T>(x);
+        const Terms<3> pt = split<3>(x);
 #pragma unroll
         for (int vt = 0; vt < VT; ++vt) {
-          Operand<T> y;
+          Terms<3> y;
 #pragma unroll
           for (int z = 0; z < N; ++z)
-            y.t[z] = *reinterpret_cast<const typename Operand<T>::V*>(&vs[z][(vt * 4 + 2 * t + s) * kTile + lane * 8]);
-          O[vt] = product32<T>(y, pt, O[vt]);
+            y.t[z] = *reinterpret_cast<const bf16x8*>(&vs[z][(vt * 4 + 2 * t + s) * kTile + lane * 8]);
+          O[vt] = product32(y, pt, O[vt]);
         }
       }
     }
@@ -308,7 +267,7 @@ __global__ __launch_bounds__(kThreads, VT == 2 ? 2 : 1) void forward(Args a) {
   }
   l += __shfl_xor(l, 32);
   if (!live) return;
-  T* p = (T*)a.o + at.rows.batch * a.ob + h * a.oh + (at.rows.first + row) * a.on;
+  float* p = (float*)a.o + at.rows.batch * a.ob + h * a.oh + (at.rows.first + row) * a.on;
 #pragma unroll
   for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
@@ -342,7 +301,7 @@ __device__ __forceinline__ int swizzle(int row) {
 // The halves of a word that are infinite or NaN, as masks of 16 bits.
 template <typename T>
 __device__ __forceinline__ unsigned not_finite(unsigned x) {
-  constexpr unsigned top = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
+  constexpr unsigned top = __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
   return (((x & 0x7fff7fffu) + top) >> 15 & 0x00010001u) * 0xffffu;
 }
 
@@ -701,7 +660,7 @@ extern "C" int kattn_fwd(const kattn_problem* p, void* o, const int64_t* o_strid
         else
           forward16<T, KS, VT, 1><<<dim3((unsigned)(a.tiles * a.H)), kThreads, 0, s>>>(a);
       else
-        forward<T, KS, VT><<<dim3((unsigned)a.tiles, a.H), kThreads, 0, s>>>(a);
+        forward<KS, VT><<<dim3((unsigned)a.tiles, a.H), kThreads, 0, s>>>(a);
     };
     if (a.Dk <= 64 && a.Dv <= 64)
       with(Int<4>(), Int<2>());

@@ -1474,8 +1474,6 @@ int64_t tiles_of(const kdelta_problem* p) {
   return p->cu_seqlens ? p->N / C + p->sequences : p->B * ((p->N + C - 1) / C);
 }
 
-int input_terms(int dtype) { return dtype == KDECAY_BF16 ? 1 : dtype == KDECAY_F16 ? 2 : 3; }
-
 int64_t blocks_of(const kdelta_problem* p) { return (p->Dv + 31) / 32; }
 
 // Wavefronts of a workgroup of chain(): four, and fewer where three terms of wide keys leave no room in

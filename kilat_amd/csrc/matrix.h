@@ -247,11 +247,6 @@ __device__ __forceinline__ TileOf tile_of(const int32_t* cu, int64_t sequences, 
   return index < 0 ? TileOf{s, 0, Rows{r.first, 0, r.batch}} : TileOf{s, index, r};  // (before the first sequence)
 }
 
-template <int C>
-inline int64_t tile_count(const int32_t* cu, int64_t B, int64_t N, int64_t sequences) {
-  return cu ? N / C + sequences : B * ((N + C - 1) / C);
-}
-
 // Zeroes columns col .. col + step*... of the rows C*tile.. of batch entry 0 that belong to no
 // sequence of a packed batch.  The tiles of a packed batch are at least as many
 // as the rows' own, so one call per tile reaches every row.
